@@ -30,6 +30,9 @@ def build(force: bool = False, verbose: bool = False, defines=(), out: str | Non
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-pthread",
            "-fno-fast-math", "-Wall", "-Wno-unused-function",
+           # no packed f32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this hardware
+           # (the host pass does not know the feature and says so: harmless)
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
            "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-x", "hip"]
     cmd += ["-Rpass-analysis=kernel-resource-usage"]  # -> lib/kernel_resources.txt (see check_resources)
     cmd += ["-D" + d for d in defines]

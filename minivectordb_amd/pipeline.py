@@ -54,10 +54,9 @@ class ResidentSearcher:
             torch.cuda.synchronize(dev)  # batches of the previous shape may still use the old buffers
         self._pipe_key = key
         self._pipe_i = 0
-        # the traversal needs all its workgroups resident at once (it is latency-bound): its stream gets
-        # the high priority so that a ready rerank never takes their place at dispatch
-        self._t_stream = torch.cuda.Stream(device=dev, priority=-1)
-        self._r_stream = torch.cuda.Stream(device=dev, priority=0)
+        # both at the default priority: work on streams of different priorities has hung on this hardware
+        self._t_stream = torch.cuda.Stream(device=dev)
+        self._r_stream = torch.cuda.Stream(device=dev)
         # whole-batch streams of submit_interleaved (the engine keeps up to 4 per-stream scratch sets)
         self._depth = depth
         self._b_streams = [torch.cuda.Stream(device=dev) for _ in range(depth)]
