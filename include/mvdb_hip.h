@@ -228,6 +228,43 @@ int mvdb_scan_many(mvdb_index *h, const int8_t *q, int nq, int k, int metric, in
 int mvdb_scan_many_dev(mvdb_index *h, const int8_t *d_q, int nq, int k, int metric, int32_t *d_out_ids,
                        int32_t *d_out_val, int32_t *d_out_count, void *stream);
 
+/* ---- microscaled 4-bit rows ------------------------------------------------- */
+/* No reference counterpart (its one quantisation is int8 with a fixed scale, mini-vector-db.ts:972-984).  Blocks of 32
+ * components share one power-of-two scale; a component is 4 bits {sign, 2 exponent, 1 mantissa} = +-{0, .5, 1, 1.5, 2, 3, 4, 6}:
+ * 4.25 bits a component, half of the int8 row, at twice the int8 rate of the matrix cores.  Meant for candidate lists: scan
+ * for more than topK, then mvdb_rerank_many on the float32 store.
+ * Packed row, mvdb_mx4_row_bytes(h) bytes for this handle's dim: nb = 2 * ceil(dim / 64) blocks of 16 bytes of codes (component
+ * 2 i of a block in the low half of its byte i), then nb scale bytes s (scale 2^(s - 127); 255 = not a number), then zeros
+ * up to a multiple of 16.  With m the largest magnitude of a block s = max(floor(log2 m) - 2, -127) + 127; a code is
+ * the nearest to x / scale, ties to even, at most 6 in magnitude.  A block with a NaN or an infinity gets s = 255: every
+ * product with it is NaN, and no scan returns it.
+ * Products are summed in f32 by the matrix cores: exact while the scales of a row lie within a few powers of two of each other
+ * (the products are small multiples of a power of two), otherwise off by an f32 rounding or two of the largest term.
+ * `_dev` entry points take 16-byte aligned packed rows, allocate nothing, do not synchronise, may be captured into a graph and run
+ * side by side on several streams (they keep nothing in the handle).  dim <= 4096, scans dim <= 1024 and k <= 128. */
+int mvdb_mx4_row_bytes(const mvdb_index *h);
+/* rows x dim components of type dtype (0 f32, 1 bf16, 2 f16), ld components from one row to the next -> packed rows */
+int mvdb_mx4_quantize_dev(mvdb_index *h, const void *d_x, int dtype, int64_t rows, int64_t ld, uint8_t *d_packed, void *stream);
+/* packed rows -> the values they stand for, rows x dim f32 */
+int mvdb_mx4_expand_dev(mvdb_index *h, const uint8_t *d_packed, int64_t rows, float *d_values, void *stream);
+/* every dot product: out[q * ldo + r], ldo >= n */
+int mvdb_mx4_product_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, float *d_out, int64_t ldo, void *stream);
+/* The k largest dot products of each query: (value desc, id asc), out_* nq x k, ids -1 and values 0 behind the count.  d_allow: bit r
+ * set = row r may be returned (ceil(n / 32) words), NULL = all.  d_ws: the caller's, 16-byte aligned, at least
+ * mvdb_mx4_scan_workspace bytes (0 for sizes that a scan refuses), not to be shared by scans that may run at the same time.  Rows
+ * follow each other without gaps; n = 0 is allowed. */
+size_t mvdb_mx4_scan_workspace(const mvdb_index *h, int nq, int n, int k);
+int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, int k, const uint32_t *d_allow,
+                           int32_t *d_out_ids, float *d_out_val, int32_t *d_out_count, void *d_ws, size_t ws_bytes, void *stream);
+/* Host forms.  quantize: packed_out / values_out may each be NULL.  attach: quantise `rows` x dim f32 rows (row id = position, as
+ * mvdb_attach_f32) into a store that the handle keeps in HBM; rows = 0 drops it.  product / scan: f32 queries against it. */
+int mvdb_mx4_quantize(mvdb_index *h, const float *x, int64_t rows, uint8_t *packed_out, float *values_out);
+int mvdb_mx4_attach(mvdb_index *h, const float *base, int64_t rows);
+int64_t mvdb_mx4_rows(const mvdb_index *h);
+int mvdb_mx4_product(mvdb_index *h, const float *q, int nq, float *out);
+int mvdb_mx4_scan_many(mvdb_index *h, const float *q, int nq, int k, const uint32_t *allow, int32_t *out_ids, float *out_val,
+                       int32_t *out_count);
+
 /* ---- top-k merge for id-range shards --------------- */
 /* Merge `parts` per-shard results (each nq x topk, ids already global) into
  * nq x topk ordered by (l2 asc, id asc).  Inputs laid out [part][nq][topk]. */

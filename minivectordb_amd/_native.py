@@ -71,6 +71,17 @@ SYMBOLS = [
     ("mvdb_dist_many", _i, [_vp, _vp, _i, _vp, _i, _i, _vp]),
     ("mvdb_scan_many", _i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
     ("mvdb_scan_many_dev", _i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    ("mvdb_mx4_row_bytes", _i, [_vp]),
+    ("mvdb_mx4_quantize_dev", _i, [_vp, _vp, _i, _i64, _i64, _vp, _vp]),
+    ("mvdb_mx4_expand_dev", _i, [_vp, _vp, _i64, _vp, _vp]),
+    ("mvdb_mx4_product_dev", _i, [_vp, _vp, _i, _vp, _i, _vp, _i64, _vp]),
+    ("mvdb_mx4_scan_workspace", _sz, [_vp, _i, _i, _i]),
+    ("mvdb_mx4_scan_many_dev", _i, [_vp, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    ("mvdb_mx4_quantize", _i, [_vp, _vp, _i64, _vp, _vp]),
+    ("mvdb_mx4_attach", _i, [_vp, _vp, _i64]),
+    ("mvdb_mx4_rows", _i64, [_vp]),
+    ("mvdb_mx4_product", _i, [_vp, _vp, _i, _vp]),
+    ("mvdb_mx4_scan_many", _i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     ("mvdb_merge_topk_dev", _i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     ("mvdb_topk_block_bytes", _sz, [_i, _i]),
     ("mvdb_merge_topk_packed_dev", _i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),

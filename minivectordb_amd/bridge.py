@@ -381,3 +381,51 @@ class HipBridge:
             self._check(self._L.mvdb_scan_many(self.handle, _ptr(q), nq, int(k), 0 if metric == "l2" else 1,
                                                _ptr(ids), _ptr(val), _ptr(cnt)))
         return ids, val, cnt
+
+    # ---- microscaled 4-bit rows (mvdb_mx4_*; no reference counterpart)
+    def mx4RowBytes(self) -> int:
+        return self._L.mvdb_mx4_row_bytes(self.handle)
+
+    def mx4Quantize(self, rows_f32):
+        """f32 rows -> (packed rows, the values they stand for)."""
+        x = self._rows(rows_f32, np.float32, "mx4Quantize")
+        packed = np.zeros((x.shape[0], self.mx4RowBytes()), np.uint8)
+        values = np.zeros_like(x)
+        with self._lock:
+            self._check(self._L.mvdb_mx4_quantize(self.handle, _ptr(x), x.shape[0], _ptr(packed), _ptr(values)))
+        return packed, values
+
+    def mx4Attach(self, base_f32) -> None:
+        """Quantise the rows (id = position) into a 4-bit store in HBM; no rows (or None) drops it."""
+        base = np.zeros((0, self._dim()), np.float32) if base_f32 is None else self._rows(base_f32, np.float32, "mx4Attach")
+        with self._lock:
+            self._check(self._L.mvdb_mx4_attach(self.handle, _ptr(base), base.shape[0]))
+
+    def mx4Rows(self) -> int:
+        return self._L.mvdb_mx4_rows(self.handle)
+
+    def mx4ProductMany(self, q_f32):
+        """Every dot product of the quantised queries with the attached 4-bit store, nq x rows f32."""
+        q = self._rows(q_f32, np.float32, "mx4ProductMany")
+        with self._lock:
+            out = np.zeros((q.shape[0], self.mx4Rows()), np.float32)
+            self._check(self._L.mvdb_mx4_product(self.handle, _ptr(q), q.shape[0], _ptr(out)))
+        return out
+
+    def mx4ScanMany(self, q_f32, k: int, allow_bitmap=None):
+        """The k (1..128) largest dot products with the attached 4-bit store -> (ids, values, counts), by (value desc, id asc); the
+        ids are a candidate list for rerankMany."""
+        q = self._rows(q_f32, np.float32, "mx4ScanMany")
+        nq = q.shape[0]
+        with self._lock:
+            allow = None
+            if allow_bitmap is not None:
+                allow = np.ascontiguousarray(allow_bitmap, np.uint32).reshape(-1)
+                need = (self.mx4Rows() + 31) // 32
+                if allow.size < need:
+                    raise MvdbError(f"allow bitmap too short: {allow.size} words for {self.mx4Rows()} rows ({need} needed)")
+            ids = np.full((nq, max(int(k), 1)), -1, np.int32)
+            val = np.zeros((nq, max(int(k), 1)), np.float32)
+            cnt = np.zeros(nq, np.int32)
+            self._check(self._L.mvdb_mx4_scan_many(self.handle, _ptr(q), nq, int(k), _ptr(allow), _ptr(ids), _ptr(val), _ptr(cnt)))
+        return ids, val, cnt

@@ -17,6 +17,7 @@
 #include "device_index.hpp"
 #include "host_graph.hpp"
 #include "mvdb_hip.h"
+#include "mx4.hpp"
 #include "rerank.hip.hpp"
 #include "scan.hip.hpp"
 #include "traverse.hip.hpp"
@@ -444,6 +445,10 @@ struct mvdb_index {
 	const float *f32_ptr = nullptr;  // pointer the rerank kernel dereferences
 	int64_t f32_rows = 0;
 
+	// microscaled 4-bit store (mvdb_mx4_attach)
+	DevBuf mx4_rows;
+	int64_t mx4_n = 0;
+
 	// scratch
 	// Per-stream scratch (kStreamSets streams at most): visited bitmaps and the intermediates of the
 	// fused query path, so that batches on different streams can be in flight together; launches on
@@ -467,7 +472,7 @@ struct mvdb_index {
 		bool busy = false;
 	} hs[kStreamSets];
 	DevBuf st_q8, st_qf, st_ids, st_dist, st_cnt, st_ctr, st_allow, st_out_ids, st_out_l2, st_out_n,
-		st_misc, prof_buf;
+		st_misc, prof_buf, st_mx4_q, st_mx4_ws;
 
 	// tuning knobs of the timed path (mvdb_set_tuning); 0 = the engine's default
 	int traverse_waves = 0;  // 0: lean kernel + replay (traverse_lean.hip.hpp); 1: the one-wave kernel that keeps the result heap in the traversal
@@ -1809,6 +1814,258 @@ int mvdb_scan_many(mvdb_index *h, const int8_t *q, int nq, int k, int metric, in
 		HIP_OK(h, hipMemcpy(out_ids, d_ids, (size_t)nq * k * 4, hipMemcpyDeviceToHost));
 		HIP_OK(h, hipMemcpy(out_val, d_val, (size_t)nq * k * 4, hipMemcpyDeviceToHost));
 	}
+	return 1;
+}
+
+// ---- microscaled 4-bit rows (kernels: mx4.hip)
+// The `_dev` entry points allocate nothing and do not synchronise, so a caller may capture them; the caller's current device
+// is left as it was.
+namespace {
+
+struct DeviceGuard {
+	int prev = -1;
+	bool ok = false;
+	explicit DeviceGuard(mvdb_index *h)
+	{
+		if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+		ok = prev == h->device || hipSetDevice(h->device) == hipSuccess;
+		if (!ok) {
+			(void)hipGetLastError();
+			h->set_error("no HIP device " + std::to_string(h->device) + " (there is no CPU fallback)");
+		}
+		if (prev == h->device) prev = -1;
+	}
+	~DeviceGuard()
+	{
+		if (prev >= 0) (void)hipSetDevice(prev);
+	}
+};
+
+int mx4_fail(mvdb_index *h, const char *fn, const std::string &what)
+{
+	h->set_error(std::string(fn) + ": " + what);
+	return 0;
+}
+
+int mx4_result(mvdb_index *h, const char *fn, hipError_t e) { return e == hipSuccess ? 1 : mx4_fail(h, fn, hipGetErrorString(e)); }
+
+bool mx4_misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// a stage's timer, but never while the stream is being captured (events of a capture say nothing)
+struct MaybeTimer {
+	std::unique_ptr<StageTimer> t;
+	MaybeTimer(mvdb_index *h, int stage, hipStream_t s)
+	{
+		hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
+		if (!h->timing || hipStreamIsCapturing(s, &c) != hipSuccess || c != hipStreamCaptureStatusNone) return;
+		t.reset(new StageTimer(h, stage, s));
+	}
+};
+
+}  // namespace
+
+int mvdb_mx4_row_bytes(const mvdb_index *h) { return mx4_row_bytes(h->cfg.dim); }
+
+int mvdb_mx4_quantize_dev(mvdb_index *h, const void *d_x, int dtype, int64_t rows, int64_t ld, uint8_t *d_packed, void *stream)
+{
+	const char *fn = "mvdb_mx4_quantize_dev";
+	if (h->cfg.dim > kMx4MaxDim) return mx4_fail(h, fn, "dim > 4096 is not supported");
+	if (dtype < 0 || dtype > 2) return mx4_fail(h, fn, "dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+	if (rows < 0) return mx4_fail(h, fn, "negative row count");
+	if (rows == 0) return 1;
+	if (ld < h->cfg.dim) return mx4_fail(h, fn, "ld is smaller than dim");
+	if (!d_x || !d_packed) return mx4_fail(h, fn, "null pointer");
+	if (reinterpret_cast<uintptr_t>(d_x) % (dtype == 0 ? 4 : 2)) return mx4_fail(h, fn, "rows are not aligned to their type");
+	if (mx4_misaligned(d_packed)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	return mx4_result(h, fn, mx4_launch_quantize(d_x, dtype, rows, h->cfg.dim, ld, d_packed, static_cast<hipStream_t>(stream)));
+}
+
+int mvdb_mx4_expand_dev(mvdb_index *h, const uint8_t *d_packed, int64_t rows, float *d_values, void *stream)
+{
+	const char *fn = "mvdb_mx4_expand_dev";
+	if (h->cfg.dim > kMx4MaxDim) return mx4_fail(h, fn, "dim > 4096 is not supported");
+	if (rows < 0) return mx4_fail(h, fn, "negative row count");
+	if (rows == 0) return 1;
+	if (!d_packed || !d_values) return mx4_fail(h, fn, "null pointer");
+	if (mx4_misaligned(d_packed)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
+	if (reinterpret_cast<uintptr_t>(d_values) % 4) return mx4_fail(h, fn, "values are not aligned to their type");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	return mx4_result(h, fn, mx4_launch_expand(d_packed, rows, h->cfg.dim, d_values, static_cast<hipStream_t>(stream)));
+}
+
+int mvdb_mx4_product_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, float *d_out, int64_t ldo, void *stream)
+{
+	const char *fn = "mvdb_mx4_product_dev";
+	if (h->cfg.dim > kMx4MaxDim) return mx4_fail(h, fn, "dim > 4096 is not supported");
+	if (nq < 0 || n < 0) return mx4_fail(h, fn, "negative row count");
+	if (nq == 0 || n == 0) return 1;
+	if (ldo < n) return mx4_fail(h, fn, "ldo is smaller than the row count");
+	if (!d_q || !d_rows || !d_out) return mx4_fail(h, fn, "null pointer");
+	if (mx4_misaligned(d_q) || mx4_misaligned(d_rows)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
+	if (reinterpret_cast<uintptr_t>(d_out) % 4) return mx4_fail(h, fn, "products are not aligned to their type");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	return mx4_result(h, fn, mx4_launch_product(d_q, nq, d_rows, n, h->cfg.dim, d_out, ldo, static_cast<hipStream_t>(stream)));
+}
+
+size_t mvdb_mx4_scan_workspace(const mvdb_index *h, int nq, int n, int k)
+{
+	(void)h;
+	return nq > 0 && n >= 0 && k > 0 && k <= kMx4ScanMaxK ? mx4_scan_workspace(nq, n, k) : 0;
+}
+
+int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, int k, const uint32_t *d_allow,
+                           int32_t *d_out_ids, float *d_out_val, int32_t *d_out_count, void *d_ws, size_t ws_bytes, void *stream)
+{
+	const char *fn = "mvdb_mx4_scan_many_dev";
+	if (h->cfg.dim > kMx4ScanMaxDim) return mx4_fail(h, fn, "dim > 1024 is not supported");
+	if (nq < 0 || n < 0) return mx4_fail(h, fn, "negative row count");
+	if (k < 1 || k > kMx4ScanMaxK) return mx4_fail(h, fn, "k must be 1..128");
+	if (nq == 0) return 1;
+	if (!d_q || (n > 0 && !d_rows) || !d_out_ids || !d_out_val || !d_out_count || !d_ws) return mx4_fail(h, fn, "null pointer");
+	if (mx4_misaligned(d_q) || mx4_misaligned(d_rows)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
+	if (mx4_misaligned(d_ws)) return mx4_fail(h, fn, "the workspace must be 16-byte aligned");
+	if (ws_bytes < mx4_scan_workspace(nq, n, k)) return mx4_fail(h, fn, "the workspace is smaller than mvdb_mx4_scan_workspace says");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	hipStream_t s = static_cast<hipStream_t>(stream);
+	MaybeTimer t(h, 3, s);
+	return mx4_result(h, fn, mx4_launch_scan(d_q, nq, d_rows, n, h->cfg.dim, k, d_allow, d_out_ids, d_out_val, d_out_count, d_ws, s));
+}
+
+int mvdb_mx4_quantize(mvdb_index *h, const float *x, int64_t rows, uint8_t *packed_out, float *values_out)
+{
+	const char *fn = "mvdb_mx4_quantize";
+	if (rows < 0) return mx4_fail(h, fn, "negative row count");
+	if (rows == 0) return 1;
+	if (!x) return mx4_fail(h, fn, "null pointer");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	const int dim = h->cfg.dim;
+	const size_t rb = mx4_row_bytes(dim);
+	const int64_t chunk = std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)dim * 4));  // 256 MB of rows at a time
+	for (int64_t r = 0; r < rows; r += chunk) {
+		const int64_t m = std::min(chunk, rows - r);
+		float *d_x = static_cast<float *>(h->st_misc.need((size_t)m * dim * 4));
+		uint8_t *d_p = static_cast<uint8_t *>(h->st_mx4_q.need((size_t)m * rb));
+		if (!d_x || !d_p) return mx4_fail(h, fn, "out of device memory (staging)");
+		HIP_OK(h, hipMemcpy(d_x, x + r * dim, (size_t)m * dim * 4, hipMemcpyHostToDevice));
+		if (!mvdb_mx4_quantize_dev(h, d_x, 0, m, dim, d_p, nullptr)) return 0;
+		if (packed_out) HIP_OK(h, hipMemcpy(packed_out + r * rb, d_p, (size_t)m * rb, hipMemcpyDeviceToHost));
+		if (values_out) {
+			if (!mvdb_mx4_expand_dev(h, d_p, m, d_x, nullptr)) return 0;
+			HIP_OK(h, hipMemcpy(values_out + r * dim, d_x, (size_t)m * dim * 4, hipMemcpyDeviceToHost));
+		}
+		HIP_OK(h, hipDeviceSynchronize());
+	}
+	return 1;
+}
+
+int mvdb_mx4_attach(mvdb_index *h, const float *base, int64_t rows)
+{
+	const char *fn = "mvdb_mx4_attach";
+	if (rows < 0 || rows > INT32_MAX) return mx4_fail(h, fn, "row count out of range");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	const int dim = h->cfg.dim;
+	const size_t rb = mx4_row_bytes(dim);
+	h->mx4_n = 0;
+	if (!base || rows == 0) return 1;
+	uint8_t *d_p = static_cast<uint8_t *>(h->mx4_rows.need((size_t)rows * rb));
+	if (!d_p) return mx4_fail(h, fn, "out of device memory (4-bit store)");
+	const int64_t chunk = std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)dim * 4));
+	for (int64_t r = 0; r < rows; r += chunk) {
+		const int64_t m = std::min(chunk, rows - r);
+		float *d_x = static_cast<float *>(h->st_misc.need((size_t)m * dim * 4));
+		if (!d_x) return mx4_fail(h, fn, "out of device memory (staging)");
+		HIP_OK(h, hipMemcpy(d_x, base + r * dim, (size_t)m * dim * 4, hipMemcpyHostToDevice));
+		if (!mvdb_mx4_quantize_dev(h, d_x, 0, m, dim, d_p + r * rb, nullptr)) return 0;
+		HIP_OK(h, hipDeviceSynchronize());
+	}
+	h->mx4_n = rows;
+	return 1;
+}
+
+int64_t mvdb_mx4_rows(const mvdb_index *h) { return h->mx4_n; }
+
+namespace {
+// host queries -> packed on the device (the null stream)
+uint8_t *mx4_stage_queries(mvdb_index *h, const char *fn, const float *q, int nq)
+{
+	const size_t bytes = (size_t)nq * h->cfg.dim * 4;
+	float *d_x = static_cast<float *>(h->st_misc.need(bytes));
+	uint8_t *d_p = static_cast<uint8_t *>(h->st_mx4_q.need((size_t)nq * mx4_row_bytes(h->cfg.dim)));
+	if (!d_x || !d_p) {
+		mx4_fail(h, fn, "out of device memory (staging)");
+		return nullptr;
+	}
+	const hipError_t e = hipMemcpy(d_x, q, bytes, hipMemcpyHostToDevice);
+	if (e != hipSuccess) {
+		mx4_fail(h, fn, hipGetErrorString(e));
+		return nullptr;
+	}
+	return mvdb_mx4_quantize_dev(h, d_x, 0, nq, h->cfg.dim, d_p, nullptr) ? d_p : nullptr;
+}
+}  // namespace
+
+int mvdb_mx4_product(mvdb_index *h, const float *q, int nq, float *out)
+{
+	const char *fn = "mvdb_mx4_product";
+	if (h->mx4_n <= 0) return mx4_fail(h, fn, "no 4-bit store attached (mvdb_mx4_attach)");
+	if (nq < 0) return mx4_fail(h, fn, "negative row count");
+	if (nq == 0) return 1;
+	if (!q || !out) return mx4_fail(h, fn, "null pointer");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	const size_t n = (size_t)h->mx4_n;
+	uint8_t *d_q = mx4_stage_queries(h, fn, q, nq);
+	if (!d_q) return 0;
+	const int64_t chunk = std::max<int64_t>(1, ((int64_t)1 << 30) / (int64_t)(n * 4));  // 1 GB of products at a time
+	for (int64_t q0 = 0; q0 < nq; q0 += chunk) {
+		const int m = (int)std::min<int64_t>(chunk, nq - q0);
+		float *d_out = static_cast<float *>(h->st_mx4_ws.need((size_t)m * n * 4));
+		if (!d_out) return mx4_fail(h, fn, "out of device memory (products)");
+		if (!mvdb_mx4_product_dev(h, d_q + q0 * mx4_row_bytes(h->cfg.dim), m, static_cast<const uint8_t *>(h->mx4_rows.p), (int)n, d_out, (int64_t)n,
+		                          nullptr))
+			return 0;
+		HIP_OK(h, hipMemcpy(out + q0 * n, d_out, (size_t)m * n * 4, hipMemcpyDeviceToHost));
+	}
+	return 1;
+}
+
+int mvdb_mx4_scan_many(mvdb_index *h, const float *q, int nq, int k, const uint32_t *allow, int32_t *out_ids, float *out_val, int32_t *out_count)
+{
+	const char *fn = "mvdb_mx4_scan_many";
+	if (h->mx4_n <= 0) return mx4_fail(h, fn, "no 4-bit store attached (mvdb_mx4_attach)");
+	if (nq < 0) return mx4_fail(h, fn, "negative row count");
+	if (k < 1 || k > kMx4ScanMaxK) return mx4_fail(h, fn, "k must be 1..128");
+	if (nq == 0) return 1;
+	if (!q || !out_ids || !out_val || !out_count) return mx4_fail(h, fn, "null pointer");
+	DeviceGuard dev(h);
+	if (!dev.ok) return 0;
+	const int n = (int)h->mx4_n;
+	uint8_t *d_q = mx4_stage_queries(h, fn, q, nq);
+	if (!d_q) return 0;
+	uint32_t *d_allow = nullptr;
+	if (allow) {
+		const size_t bytes = ((size_t)n + 31) / 32 * 4;
+		d_allow = static_cast<uint32_t *>(h->st_allow.need(bytes));
+		if (!d_allow) return mx4_fail(h, fn, "out of device memory (staging)");
+		HIP_OK(h, hipMemcpy(d_allow, allow, bytes, hipMemcpyHostToDevice));
+	}
+	const size_t ws = mx4_scan_workspace(nq, n, k), cells = (size_t)nq * k * 4;
+	int32_t *d_ids = static_cast<int32_t *>(h->st_ids.need(cells));
+	float *d_val = static_cast<float *>(h->st_dist.need(cells));
+	int32_t *d_cnt = static_cast<int32_t *>(h->st_cnt.need((size_t)nq * 4));
+	void *d_ws = h->st_mx4_ws.need(ws);
+	if (!d_ids || !d_val || !d_cnt || !d_ws) return mx4_fail(h, fn, "out of device memory (scan staging)");
+	if (!mvdb_mx4_scan_many_dev(h, d_q, nq, static_cast<const uint8_t *>(h->mx4_rows.p), n, k, d_allow, d_ids, d_val, d_cnt, d_ws, ws, nullptr)) return 0;
+	HIP_OK(h, hipMemcpy(out_ids, d_ids, cells, hipMemcpyDeviceToHost));
+	HIP_OK(h, hipMemcpy(out_val, d_val, cells, hipMemcpyDeviceToHost));
+	HIP_OK(h, hipMemcpy(out_count, d_cnt, (size_t)nq * 4, hipMemcpyDeviceToHost));
 	return 1;
 }
 

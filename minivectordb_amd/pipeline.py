@@ -12,7 +12,7 @@ import ctypes as C
 
 import torch
 
-from .bridge import HipBridge
+from .bridge import HipBridge, MvdbError
 from .distributed import TopkBlock
 
 
@@ -208,3 +208,106 @@ class ResidentSearcher:
         launches, total = C.c_longlong(0), C.c_double(0.0)
         self.L.mvdb_stage_stats(self.h, int(stage), C.byref(launches), C.byref(total), 1 if reset else 0)
         return launches.value, total.value
+
+
+class ResidentMx4:
+    """The microscaled 4-bit operators over device tensors (mvdb_mx4_*_dev; the format is in include/mvdb_hip.h): rows -> packed
+    rows, packed rows -> values, every dot product, the k largest dot products.  Everything runs on the caller's current
+    stream of `device`; nothing is kept between calls and nothing synchronises, so calls may be captured into a graph."""
+
+    _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+    def __init__(self, bridge: HipBridge, device: torch.device):
+        self.b, self.L = bridge, bridge._L
+        bridge.handle  # an initialised bridge is needed
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise MvdbError(f"ResidentMx4: a GPU device is needed, got {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+
+    @property
+    def dim(self) -> int:
+        return self.b._dim()
+
+    @property
+    def row_bytes(self) -> int:
+        return self.b.mx4RowBytes()
+
+    def _stream(self):
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _on_device(self, t, what: str):
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise MvdbError(f"{what}: a tensor on {self.device} is needed, got {getattr(t, 'device', type(t).__name__)}")
+
+    def _packed(self, t, what: str):
+        self._on_device(t, what)
+        if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != self.row_bytes or not t.is_contiguous():
+            raise MvdbError(f"{what}: packed rows are contiguous uint8 [rows, {self.row_bytes}], got {t.dtype} {tuple(t.shape)}")
+        if t.shape[0] > 2**31 - 1:
+            raise MvdbError(f"{what}: {t.shape[0]} rows, at most 2^31 - 1")
+        return t
+
+    def quantize(self, x: torch.Tensor) -> torch.Tensor:
+        """[rows, dim] f32, bf16 or f16 (rows may lie apart, components may not) -> packed rows, uint8 [rows, row_bytes]."""
+        self._on_device(x, "mx4 quantize")
+        if x.dtype not in self._DTYPES:
+            raise MvdbError(f"mx4 quantize: float32, bfloat16 or float16 rows are needed, got {x.dtype}")
+        if x.dim() != 2 or x.shape[1] != self.dim:
+            raise MvdbError(f"mx4 quantize: expected rows of dim={self.dim}, got shape {tuple(x.shape)}")
+        rows = x.shape[0]
+        ld = x.stride(0) if rows > 1 else self.dim
+        if x.stride(1) != 1 or ld < self.dim:
+            raise MvdbError(f"mx4 quantize: components have to follow each other and rows not overlap, got strides {x.stride()}")
+        out = torch.empty((rows, self.row_bytes), dtype=torch.uint8, device=self.device)
+        self.b._check(self.L.mvdb_mx4_quantize_dev(self.b.handle, C.c_void_p(x.data_ptr()), self._DTYPES[x.dtype], rows, ld,
+                                                   C.c_void_p(out.data_ptr()), self._stream()))
+        return out
+
+    def expand(self, packed: torch.Tensor) -> torch.Tensor:
+        """Packed rows -> the values they stand for, f32 [rows, dim]."""
+        self._packed(packed, "mx4 expand")
+        out = torch.empty((packed.shape[0], self.dim), dtype=torch.float32, device=self.device)
+        self.b._check(self.L.mvdb_mx4_expand_dev(self.b.handle, C.c_void_p(packed.data_ptr()), packed.shape[0], C.c_void_p(out.data_ptr()),
+                                                 self._stream()))
+        return out
+
+    def product(self, q: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Every dot product of packed queries and packed rows, f32 [nq, n]; `out` may be a slice with wider rows."""
+        self._packed(q, "mx4 product (queries)")
+        self._packed(rows, "mx4 product (rows)")
+        nq, n = q.shape[0], rows.shape[0]
+        if out is None:
+            out = torch.empty((nq, n), dtype=torch.float32, device=self.device)
+        self._on_device(out, "mx4 product (out)")
+        ldo = out.stride(0) if nq > 1 and out.dim() == 2 else n
+        if out.dtype != torch.float32 or tuple(out.shape) != (nq, n) or (n > 1 and out.stride(1) != 1) or ldo < n:
+            raise MvdbError(f"mx4 product: out has to be float32 [{nq}, {n}] with rows in one piece that do not overlap, got {out.dtype} "
+                            f"{tuple(out.shape)} strides {out.stride()}")
+        self.b._check(self.L.mvdb_mx4_product_dev(self.b.handle, C.c_void_p(q.data_ptr()), nq, C.c_void_p(rows.data_ptr()), n,
+                                                  C.c_void_p(out.data_ptr()), ldo, self._stream()))
+        return out
+
+    def scan_many(self, q: torch.Tensor, rows: torch.Tensor, k: int, allow: torch.Tensor | None = None):
+        """The k (1..128) largest dot products of each packed query -> (ids i32 [nq, k], values f32 [nq, k], counts i32 [nq]) by (value
+        desc, id asc); ids -1 and values 0 behind the count.  allow: bitmap over the rows (int32 words) or None."""
+        self._packed(q, "mx4 scan (queries)")
+        self._packed(rows, "mx4 scan (rows)")
+        nq, n, k = q.shape[0], rows.shape[0], int(k)
+        if allow is not None:
+            self._on_device(allow, "mx4 scan (allow)")
+            if allow.dtype not in (torch.int32, torch.uint32) or allow.dim() != 1 or not allow.is_contiguous() or allow.shape[0] < (n + 31) // 32:
+                raise MvdbError(f"mx4 scan: allow is a bitmap of at least {(n + 31) // 32} int32 words, got {allow.dtype} {tuple(allow.shape)}")
+        if not 1 <= k <= 128:
+            raise MvdbError(f"mx4 scan: k must be 1..128, got {k}")
+        ids = torch.empty((nq, k), dtype=torch.int32, device=self.device)
+        val = torch.empty((nq, k), dtype=torch.float32, device=self.device)
+        cnt = torch.empty((nq,), dtype=torch.int32, device=self.device)
+        need = self.L.mvdb_mx4_scan_workspace(self.b.handle, nq, n, k)
+        ws = torch.empty((need,), dtype=torch.uint8, device=self.device)
+        vp = C.c_void_p
+        self.b._check(self.L.mvdb_mx4_scan_many_dev(self.b.handle, vp(q.data_ptr()), nq, vp(rows.data_ptr()), n, k,
+                                                    vp(allow.data_ptr()) if allow is not None else None, vp(ids.data_ptr()),
+                                                    vp(val.data_ptr()), vp(cnt.data_ptr()), vp(ws.data_ptr()), need, self._stream()))
+        return ids, val, cnt
