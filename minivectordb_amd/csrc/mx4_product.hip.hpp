@@ -22,21 +22,24 @@ __device__ __forceinline__ mx4_v16f mx4_mfma(const mx4_v4i &a, int sa, const mx4
 	return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, OA, sa, OB, sb);
 }
 
-// A wave computes 64 queries x 64 rows, a workgroup (2 x 2 waves) 128 x 128; fragments come straight from memory.
+// A wave computes 64 queries x 64 rows, a workgroup (2 x 2 waves) 128 x 128; fragments come straight from memory.  Column c of the
+// result is row c, or (step > 1) row 64 * step * (c / 64) + c % 64: the 64-row tiles that are multiples of step.  Columns past the
+// last row hold products that nobody reads.
 __global__ __launch_bounds__(256) void mx4_product_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, float *out,
-                                                          int64_t ldo, int qtiles)
+                                                          int64_t ldo, int qtiles, int cols, int64_t step)
 {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 	const int half = lane >> 5, r32 = lane & 31;
 	const int qt = blockIdx.x % qtiles, rt = blockIdx.x / qtiles;
 	const int q0 = qt * 128 + (wave >> 1) * 64, r0 = rt * 128 + (wave & 1) * 64;
-	if (q0 >= nq || r0 >= n) return;
+	if (q0 >= nq || r0 >= cols) return;
 	const uint8_t *qp[2], *rp[2];
 #pragma unroll
 	for (int t = 0; t < 2; t++) {
-		const int qi = q0 + t * 32 + r32, ri = r0 + t * 32 + r32;
+		const int qi = q0 + t * 32 + r32, col = r0 + t * 32 + r32;
+		const int64_t ri = col + (int64_t)(col & ~63) * (step - 1);
 		qp[t] = q + (int64_t)(qi < nq ? qi : nq - 1) * row_bytes;
-		rp[t] = rows + (int64_t)(ri < n ? ri : n - 1) * row_bytes;
+		rp[t] = rows + (ri < n ? ri : n - 1) * row_bytes;
 	}
 	mx4_v16f acc[2][2];
 #pragma unroll
@@ -65,30 +68,38 @@ __global__ __launch_bounds__(256) void mx4_product_kernel(const uint8_t *q, int 
 	for (int t = 0; t < 2; t++)
 #pragma unroll
 		for (int u = 0; u < 2; u++) {
-			const int ri = r0 + u * 32 + r32;
+			const int col = r0 + u * 32 + r32;
 #pragma unroll
 			for (int i = 0; i < 16; i++) {
 				const int qi = q0 + t * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-				if (qi < nq && ri < n) out[qi * ldo + ri] = acc[t][u][i];
+				if (qi < nq && col < cols) out[qi * ldo + col] = acc[t][u][i];
 			}
 		}
 }
 
-hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, float *out, int64_t ldo, hipStream_t s)
+// `cols` columns
+inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8_t *rows, int n, int cols, int64_t step, int ksteps, int row_bytes, float *out,
+                                           int64_t ldo, hipStream_t s)
 {
-	const int rb = mx4_row_bytes(dim), ks = mx4_blocks(dim) / 2;
-	const int64_t rtiles = ((int64_t)n + 127) / 128;
-	const int64_t step = 1 << 16;  // queries a launch (what one grid can hold)
-	for (int64_t q0 = 0; q0 < nq; q0 += step) {
-		const int m = (int)(nq - q0 < step ? nq - q0 : step), qtiles = (m + 127) / 128;
+	const int64_t rtiles = ((int64_t)cols + 127) / 128;
+	const int64_t qstep = 1 << 16;  // queries a launch (what one grid can hold)
+	for (int64_t q0 = 0; q0 < nq; q0 += qstep) {
+		const int m = (int)(nq - q0 < qstep ? nq - q0 : qstep), qtiles = (m + 127) / 128;
 		const int64_t rstep = ((int64_t)1 << 22) / qtiles;
 		for (int64_t r0 = 0; r0 < rtiles; r0 += rstep) {
 			const int64_t c = rtiles - r0 < rstep ? rtiles - r0 : rstep;
-			hipLaunchKernelGGL(mx4_product_kernel, dim3((unsigned)(c * qtiles)), dim3(256), 0, s, q + q0 * rb, m, rows + r0 * 128 * rb,
-			                   (int)(n - r0 * 128), ks, rb, out + q0 * ldo + r0 * 128, ldo, qtiles);
+			const int64_t col = r0 * 128, row = col * step;
+			if (row >= n) break;
+			hipLaunchKernelGGL(mx4_product_kernel, dim3((unsigned)(c * qtiles)), dim3(256), 0, s, q + q0 * row_bytes, m, rows + row * row_bytes,
+			                   (int)(n - row), ksteps, row_bytes, out + q0 * ldo + col, ldo, qtiles, (int)(cols - col), step);
 		}
 	}
 	return hipGetLastError();
+}
+
+hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, float *out, int64_t ldo, hipStream_t s)
+{
+	return mx4_launch_product_tiles(q, nq, rows, n, n, 1, mx4_blocks(dim) / 2, mx4_row_bytes(dim), out, ldo, s);
 }
 
 }  // namespace mvdb
