@@ -14,13 +14,15 @@
 // ratio^L-th tile, level l the tiles that are multiples of ratio^(L - l) and not of ratio^(L - l + 1).  After a level the k-th best key so
 // far is a bound: k rows are at least that good, so only keys above it matter, and as the rows seen so far are spread evenly over the
 // store about k (ratio - 1) keys of the next level are (whatever order the rows are in, unless they repeat with the tiles' period).
-// Level 0 has no bound: its products go to memory.  From then on a product that passes the bound is pushed into a queue of its wave in LDS, and
-// from there into the query's buffer of kMx4Cap keys; mx4_pick_kernel cuts the buffer to its best k after every level.  A buffer that
-// overflows marks its query, and mx4_rescue_kernel does those over, one workgroup each.
+// Level 0 has no bound: its products go to memory.  From then on a lane whose product passes the bound appends the key to a list of its
+// own, which needs no atomics: a lane only ever sees one query a fragment, and the tiles are dealt out in turn, so lists stay short.
+// mx4_pick_kernel gathers a query's lists after every level and keeps the best k.  A list that overflows marks its query, and
+// mx4_rescue_kernel does those over, one workgroup each.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "mx4.hpp"
@@ -185,9 +187,6 @@ __device__ void mx4_block_topk(F key_at, int m, int k, int64_t q, int64_t stride
 	}
 }
 
-// Rows of level 0 and of a level's tile i.  step = ratio^(L - l); tiles of level l >= 1: step * (i + i / (ratio - 1) + 1).
-__host__ __device__ inline int64_t mx4_level_tile(int64_t i, int64_t step, int ratio) { return ratio ? step * (i + i / (ratio - 1) + 1) : step * i; }
-
 // one workgroup per query: the best k of level 0's products (m of them, product j belongs to row (j / 64) * 64 * step + j % 64)
 __global__ __launch_bounds__(256) void mx4_pick_first_kernel(const float *scores, int m, int64_t step, int n, int k, const uint32_t *allow, Mx4Out o,
                                                              int64_t stride, int32_t *over)
@@ -205,22 +204,53 @@ __global__ __launch_bounds__(256) void mx4_pick_first_kernel(const float *scores
 	mx4_block_topk<256>(key_at, m, k, q, stride, o, l, best);
 }
 
-// one workgroup per query: the best k of its buffer
-template <int T>
-__global__ __launch_bounds__(T) void mx4_pick_kernel(const mx4_key *keys, const int32_t *fill, int cap, int k, Mx4Out o, int32_t *over)
+// one workgroup per query: the best k of the `m` keys that the chunks left (0 = none)
+__global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *keys, int m, int k, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
 	__shared__ mx4_key best[kMx4ScanMaxK];
 	const int64_t q = blockIdx.x;
-	const mx4_key *mine = keys + q * cap;
-	int m = fill ? fill[q] : cap;
-	if (m > cap) {  // keys were lost
-		m = cap;
-		if (threadIdx.x == 0) over[q] = 1;
-	}
-	if (o.keys) __syncthreads();  // fill[q] has been read by everybody before it is written
+	const mx4_key *mine = keys + q * m;
 	auto key_at = [&](int j) -> mx4_key { return mine[j]; };
-	mx4_block_topk<T>(key_at, m, k, q, cap, o, l, best);
+	mx4_block_topk<1024>(key_at, m, k, q, 0, o, l, best);
+}
+
+// one workgroup per query: the best k of what it had and of its lists
+constexpr int kMx4List = 64;       // keys of a list
+constexpr int kMx4Gather = 2048;   // keys of all lists of a query
+
+__global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, const int32_t *counts, int parts, const mx4_key *before, const int32_t *nbefore,
+                                                       int k, Mx4Out o, int32_t *over)
+{
+	__shared__ Mx4PickLds l;
+	__shared__ mx4_key best[kMx4ScanMaxK], keys[kMx4Gather];
+	__shared__ int total, lost;
+	const int64_t q = blockIdx.x;
+	const int tid = threadIdx.x, had = nbefore[q];
+	if (tid == 0) {
+		total = had;
+		lost = 0;
+	}
+	for (int i = tid; i < had; i += 256) keys[i] = before[q * kMx4ScanMaxK + i];
+	__syncthreads();
+	for (int i = tid; i < parts; i += 256) {
+		int c = counts[q * parts + i];
+		if (c > 0) {
+			if (c > kMx4List) {
+				lost = 1;
+				c = kMx4List;
+			}
+			const int at = atomicAdd(&total, c);
+			const mx4_key *src = lists + (q * parts + i) * kMx4List;
+			for (int j = 0; j < c; j++)
+				if (at + j < kMx4Gather) keys[at + j] = src[j];
+		}
+	}
+	__syncthreads();
+	const int m = total < kMx4Gather ? total : kMx4Gather;
+	if (tid == 0 && (lost || total > kMx4Gather)) over[q] = 1;
+	auto key_at = [&](int j) -> mx4_key { return keys[j]; };
+	mx4_block_topk<256>(key_at, m, k, q, kMx4ScanMaxK, o, l, best);
 }
 
 // ---------------------------------------------------------------------------------------------- queries in registers
@@ -330,120 +360,283 @@ __global__ __launch_bounds__(256) void mx4_chunk_kernel(const uint8_t *q, int nq
 }
 
 // ---------------------------------------------------------------------------------------------- levels
-constexpr int kMx4Cap = 2048;      // keys of a query's buffer
 constexpr int kMx4FirstTiles = 16;  // 64-row tiles of level 0, at most
-constexpr int kMx4Queue = 192;     // keys of a wave's queue
 
 struct Mx4Level {
 	const uint8_t *q, *rows;
 	const uint32_t *allow;
 	int nq, n, ksteps, row_bytes;
-	int64_t step;    // see mx4_level_tile
-	int ratio, tiles;
-	mx4_key *keys;   // [nq][kMx4Cap]
-	int32_t *fill;   // [nq] keys in the buffer (may run past kMx4Cap)
+	int64_t step;     // see mx4_level_tile
+	unsigned skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
+	int tiles;
 	const mx4_key *bound;  // [nq], 0 = none
+	mx4_key *lists;   // [nq][parts][kMx4List]
+	int32_t *counts;  // [nq][parts] keys of a list (may run past kMx4List)
+	int parts;
 };
 
-// A wave's queue of candidates
-struct Mx4Queue {
-	mx4_key key[kMx4Queue];
-	int q[kMx4Queue];
-};
-
-// Empty the queue: one atomic per key, 64 in flight.
-__device__ __forceinline__ void mx4_flush(const Mx4Level &a, Mx4Queue &w, int &n, int lane)
+// tile i of a level, first row: i / (ratio - 1) by a multiplication, exact for i (ratio - 1) < 2^32 (i < 2^25)
+__device__ __forceinline__ int64_t mx4_tile_row(const Mx4Level &a, unsigned i)
 {
-	asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-	for (int i = lane; i < n; i += 64) {
-		const mx4_key key = w.key[i];
-		const int q = w.q[i];
-		const int slot = atomicAdd(&a.fill[q], 1);
-		if (slot < kMx4Cap) a.keys[(int64_t)q * kMx4Cap + slot] = key;
-	}
-	asm volatile("" ::: "memory");
-	n = 0;
+	if (a.skip) i += (unsigned)(((uint64_t)i * a.skip) >> 32) + 1;
+	return (int64_t)i * a.step * 64;
 }
 
-// Candidates of one 32 x 32 tile: rows row0 .. + 31, query `q` in this lane's column
-__device__ __forceinline__ void mx4_push(const Mx4Level &a, const mx4_v16f &acc, float bound, mx4_key bkey, int q, int64_t row0, int half, int lane, Mx4Queue &w,
-                                         int &n)
+// a word of the filter at a place that all lanes agree on, through the scalar cache (a vector load would wait for the LDS-DMA loads before it)
+__device__ __forceinline__ uint32_t mx4_allow_word(const uint32_t *allow, int64_t at)
+{
+	using const_ptr_t = const __attribute__((address_space(4))) uint32_t *;
+	return ((const_ptr_t)(allow))[at];
+}
+
+// 64 queries of a wave: two fragments of 32, and for each this lane's query, its bound and its list
+template <int KS>
+struct Mx4Queries {
+	Mx4Frag<KS> b[2];
+	float bound[2];
+	mx4_key bkey[2];
+	unsigned list[2];  // index of the list's first key
+	int count[2];
+};
+
+template <int KS, bool EXACT>
+__device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS> &w, const Mx4Level &a, int q0, int part, int half, int r32, int ksteps, int row_bytes)
 {
 #pragma unroll
-	for (int i = 0; i < 16; i++) {
-		if (__ballot(acc[i] >= bound)) {
-			const mx4_key key = mx4_make_key(acc[i], (unsigned)(row0 + 8 * (i >> 2) + 4 * half + (i & 3)));
-			const bool p = acc[i] >= bound && key > bkey;
-			const unsigned long long who = __ballot(p);
-			if (n + 64 > kMx4Queue) mx4_flush(a, w, n, lane);
-			if (p) {
-				const int at = n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
-				w.key[at] = key;
-				w.q[at] = q;
-			}
-			n += __popcll(who);
+	for (int c = 0; c < 2; c++) {
+		const int q = q0 + c * 32 + r32, qs = q < a.nq ? q : a.nq - 1;
+		mx4_load_frag<KS, EXACT>(w.b[c], a.q + (int64_t)qs * row_bytes, half, ksteps);
+		mx4_shift_scales(w.b[c], half);
+		w.bkey[c] = a.bound[qs];
+		// no query in this column: nothing is >= NaN
+		w.bound[c] = q >= a.nq ? __uint_as_float(0x7fc00000u) : w.bkey[c] ? mx4_key_value(w.bkey[c]) : -__builtin_inff();
+		w.list[c] = ((unsigned)qs * a.parts + part) * kMx4List;
+		w.count[c] = 0;
+	}
+}
+template <int KS>
+__device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS> &w, const Mx4Level &a, int q0, int part, int r32)
+{
+#pragma unroll
+	for (int c = 0; c < 2; c++)
+		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = w.count[c];
+}
+
+// Products of 32 rows (row0 ..) with the wave's queries: test, and append what passes.  The test is one maximum over the lane's 16 rows; who
+// passed is looked for four rows at a time.
+template <int KS>
+__device__ __forceinline__ void mx4_test(Mx4Queries<KS> &w, const Mx4Level &a, const mx4_v16f (&acc)[2], int64_t row0, int half)
+{
+#pragma unroll
+	for (int c = 0; c < 2; c++) {
+		float m[4];
+#pragma unroll
+		for (int g = 0; g < 4; g++) m[g] = __builtin_fmaxf(__builtin_fmaxf(acc[c][4 * g], acc[c][4 * g + 1]), __builtin_fmaxf(acc[c][4 * g + 2], acc[c][4 * g + 3]));
+		const float top = __builtin_fmaxf(__builtin_fmaxf(m[0], m[1]), __builtin_fmaxf(m[2], m[3]));
+		if (__builtin_expect(__ballot(top >= w.bound[c]) != 0, 0)) {
+			unsigned id0 = (unsigned)row0 + 4 * half;
+			asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
+#pragma unroll
+			for (int g = 0; g < 4; g++)
+				if (__ballot(m[g] >= w.bound[c])) {
+#pragma unroll
+					for (int j = 0; j < 4; j++) {
+						const float v = acc[c][4 * g + j];
+						if (v >= w.bound[c]) {
+							const mx4_key key = mx4_make_key(v, id0 + 8 * g + j);
+							if (key > w.bkey[c]) {
+								if (w.count[c] < kMx4List) a.lists[(size_t)w.list[c] + w.count[c]] = key;
+								w.count[c]++;
+							}
+						}
+					}
+				}
 		}
 	}
 }
 
-// Independent waves: each holds 64 queries and takes every (waves)-th half tile of the level straight from memory.
+// Independent waves: each holds 64 queries and takes every (waves)-th half tile of the level straight from memory, the next one's rows under
+// way while it multiplies.
 template <int KS, bool EXACT>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgroups)
 {
-	__shared__ Mx4Queue queue[4];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
-	const int gw = blockIdx.x * 4 + wave, group = gw % qgroups;
-	const int64_t first = gw / qgroups, waves = (int64_t)gridDim.x * 4 / qgroups;  // (the grid is a multiple of qgroups waves)
+	const int gw = blockIdx.x * 4 + wave, group = gw % qgroups, waves = a.parts / 2, first = gw / qgroups;
 	if (first >= waves) return;
-	Mx4Queue &w = queue[wave];
-	int qn = 0;
-	Mx4Frag<KS> b[2];
-	float bound[2];
-	mx4_key bkey[2];
-	int qi[2];
-#pragma unroll
-	for (int c = 0; c < 2; c++) {
-		qi[c] = group * 64 + c * 32 + r32;
-		const int qs = qi[c] < a.nq ? qi[c] : a.nq - 1;
-		mx4_load_frag<KS, EXACT>(b[c], a.q + (int64_t)qs * a.row_bytes, half, a.ksteps);
-		mx4_shift_scales(b[c], half);
-		bkey[c] = a.bound[qs];
-		// no query in this column: nothing is >= NaN
-		bound[c] = qi[c] >= a.nq ? __uint_as_float(0x7fc00000u) : bkey[c] ? mx4_key_value(bkey[c]) : -__builtin_inff();
-	}
-	for (int64_t i = first; i < 2 * (int64_t)a.tiles; i += waves) {
-		const int64_t row0 = mx4_level_tile(i >> 1, a.step, a.ratio) * 64 + (i & 1) * 32;
-		if (row0 >= a.n) continue;
-		unsigned keep = row0 + 32 <= a.n ? 0xffffffffu : (1u << (a.n - row0)) - 1u;
-		if (a.allow) keep &= a.allow[row0 >> 5];
-		if (keep == 0) continue;
+	const int row_bytes = EXACT ? 32 * KS + (2 * KS + 15) / 16 * 16 : a.row_bytes, ksteps = EXACT ? KS : a.ksteps;
+	Mx4Queries<KS> w;
+	mx4_load_queries<KS, EXACT>(w, a, group * 64, 2 * first + half, half, r32, ksteps, row_bytes);
+	const unsigned total = 2 * (unsigned)a.tiles;
+	// half tile i: its first row and which of its rows count, and (unless none does) the rows
+	auto load = [&](unsigned i, Mx4Frag<KS> &f, int64_t &row0, unsigned &keep) {
+		row0 = mx4_tile_row(a, i >> 1) + (i & 1) * 32;
+		keep = 0;
+		if (row0 >= a.n) return;
+		keep = row0 + 32 <= a.n ? 0xffffffffu : (1u << (a.n - row0)) - 1u;
+		if (a.allow) keep &= mx4_allow_word(a.allow, row0 >> 5);
+		if (keep == 0) return;
 		const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
-		Mx4Frag<KS> f;
-		mx4_load_frag<KS, EXACT>(f, a.rows + r * a.row_bytes, half, a.ksteps);
+		mx4_load_frag<KS, EXACT>(f, a.rows + r * row_bytes, half, ksteps);
+	};
+	auto use = [&](Mx4Frag<KS> &f, int64_t row0, unsigned keep) {
+		if (keep == 0) return;
 		const bool out = !((keep >> r32) & 1u);
 #pragma unroll
 		for (int s = 0; s < (KS + 1) / 2; s++) f.sc[s] = out ? -1 : f.sc[s];
 		mx4_shift_scales(f, half);
 		mx4_v16f acc[2];
-		mx4_tile<KS, EXACT, 2>(f, b, a.ksteps, acc);
-#pragma unroll
-		for (int c = 0; c < 2; c++) {
-			float m = acc[c][0];
-#pragma unroll
-			for (int j = 1; j < 16; j++) m = __builtin_fmaxf(m, acc[c][j]);
-			if (__ballot(m >= bound[c])) mx4_push(a, acc[c], bound[c], bkey[c], qi[c], row0, half, lane, w, qn);
+		mx4_tile<KS, EXACT, 2>(f, w.b, ksteps, acc);
+		mx4_test(w, a, acc, row0, half);
+	};
+	if constexpr (KS <= 8) {
+		Mx4Frag<KS> f0, f1;
+		int64_t row0, row1;
+		unsigned keep0 = 0, keep1 = 0;
+		unsigned i = first;
+		if (i < total) load(i, f0, row0, keep0);
+		while (i < total) {
+			keep1 = 0;
+			if (i + waves < total) load(i + waves, f1, row1, keep1);
+			__builtin_amdgcn_sched_barrier(0);
+			use(f0, row0, keep0);
+			i += waves;
+			if (i >= total) break;
+			keep0 = 0;
+			if (i + waves < total) load(i + waves, f0, row0, keep0);
+			__builtin_amdgcn_sched_barrier(0);
+			use(f1, row1, keep1);
+			i += waves;
+		}
+	} else {
+		for (unsigned i = first; i < total; i += waves) {
+			Mx4Frag<KS> f;
+			int64_t row0;
+			unsigned keep;
+			load(i, f, row0, keep);
+			use(f, row0, keep);
 		}
 	}
-	mx4_flush(a, w, qn, lane);
+	mx4_store_counts(w, a, group * 64, 2 * first + half, r32);
 }
 
-// The queries whose buffer overflowed, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
+// 64 consecutive rows a tile, staged in LDS for up to 8 waves of 64 queries each.  The tiles come by LDS-DMA into a ring of four, three tiles
+// ahead; one barrier a tile: after it tile t + 1 is there for everybody and the place of tile t - 1 is free.  An image row is the packed
+// row, plus one slot of 16 bytes where that makes the stride an odd number of slots: then the 16 lanes that an LDS read serves at a time hit
+// 16 different slots.  Two waves a SIMD: one tests while the other multiplies.
+constexpr int kMx4Ring = 4;
+static __device__ __align__(16) int g_mx4_nan[4] = {-1, -1, -1, -1};  // scales 255: the blocks of a row that is left out
+
+__host__ __device__ constexpr int mx4_image_slots(int row_bytes) { return (row_bytes / 16) | 1; }
+
+template <int N>
+__device__ __forceinline__ void mx4_wait_vm()
+{
+	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// until at most n vector-memory operations of this wave are outstanding (n is wave-uniform); more than 6 counts as 0
+__device__ __forceinline__ void mx4_wait_vm_upto(int n)
+{
+	switch (n) {
+	case 1: mx4_wait_vm<1>(); break;
+	case 2: mx4_wait_vm<2>(); break;
+	case 3: mx4_wait_vm<3>(); break;
+	case 4: mx4_wait_vm<4>(); break;
+	case 5: mx4_wait_vm<5>(); break;
+	case 6: mx4_wait_vm<6>(); break;
+	default: mx4_wait_vm<0>(); break;
+	}
+}
+
+template <int KS, bool EXACT>
+__global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtiles, int splits)
+{
+	extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
+	const int nwaves = blockDim.x >> 6;
+	// blocks with equal blockIdx % 8 share an XCD and its L2: they take the same tiles for their different queries
+	const int j8 = blockIdx.x >> 3, qtile = j8 % qtiles;
+	const int split = (blockIdx.x & 7) + 8 * (j8 / qtiles);
+	const int row_bytes = EXACT ? 32 * KS + (2 * KS + 15) / 16 * 16 : a.row_bytes, ksteps = EXACT ? KS : a.ksteps;
+	const int slots = row_bytes / 16, islots = slots | 1;
+	const int tile_bytes = islots * 64 * 16;
+	const int q0 = (qtile * nwaves + wave) * 64;
+	Mx4Queries<KS> w;
+	mx4_load_queries<KS, EXACT>(w, a, q0, 2 * split + half, half, r32, ksteps, row_bytes);
+	const int ntiles = split < a.tiles ? (a.tiles - split + splits - 1) / splits : 0;
+
+	using lds_ptr_t = __attribute__((address_space(3))) void *;
+	using glb_ptr_t = __attribute__((address_space(1))) const void *;
+	// this wave's share of tile t: instructions wave, wave + nwaves, ... of islots, 64 slots of 16 bytes each
+	auto fetch = [&](int t) {
+		const int64_t row0 = mx4_tile_row(a, split + t * splits);
+		const uint8_t *base = a.rows + row0 * row_bytes;
+		unsigned char *dst = lds + (t & (kMx4Ring - 1)) * tile_bytes;
+		if (islots == slots && !a.allow && row0 + 64 <= a.n) {  // the image is the tile as it lies in memory
+			for (int i = wave; i < islots; i += nwaves)
+				__builtin_amdgcn_global_load_lds((glb_ptr_t)(base + i * 1024 + (unsigned)lane * 16), (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
+			return;
+		}
+		uint64_t keep = row0 + 64 <= a.n ? ~0ull : (1ull << (a.n - row0)) - 1;
+		if (a.allow) {
+			const uint64_t lo = mx4_allow_word(a.allow, row0 >> 5), hi = row0 + 32 < a.n ? mx4_allow_word(a.allow, (row0 >> 5) + 1) : 0u;
+			keep &= lo | (hi << 32);
+		}
+		for (int i = wave; i < islots; i += nwaves) {
+			const int slot = i * 64 + lane;
+			const int r = slot / islots, pos = slot - r * islots;
+			const void *src = base + (r * slots + (pos < slots ? pos : 0)) * 16;
+			// a row that is left out has scales 255; past the last row nothing is read
+			const bool off = !((keep >> r) & 1) && (pos >= 2 * ksteps || row0 + r >= a.n);
+			src = off ? static_cast<const void *>(g_mx4_nan) : src;
+			__builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
+		}
+	};
+	const int mine = (islots - wave + nwaves - 1) / nwaves;  // instructions of a fetch by this wave
+	auto image = [&](int t, int h) -> const unsigned char * { return lds + (t & (kMx4Ring - 1)) * tile_bytes + (h * 32 + r32) * islots * 16; };
+	mx4_wait_vm<0>();
+	for (int t = 0; t < 3 && t < ntiles; t++) fetch(t);
+	mx4_wait_vm_upto(ntiles > 2 && 2 * mine <= 6 ? 2 * mine : 0);  // this wave's share of tile 0
+	__builtin_amdgcn_s_barrier();
+	asm volatile("" ::: "memory");
+	constexpr bool AHEAD = KS <= 8;  // room in the registers for the fragments of the next 32 rows
+	Mx4Frag<KS> f0, f1;
+	if (AHEAD && ntiles > 0) mx4_load_frag<KS, EXACT>(f0, image(0, 0), half, ksteps);
+	for (int t = 0; t < ntiles; t++) {
+		// this wave's share of tile t + 1 is there (loads complete in order; the share of tile t + 2 may be under way) ...
+		mx4_wait_vm_upto(t + 2 < ntiles ? mine : 0);
+		__builtin_amdgcn_s_barrier();  // ... and everybody's, and tile t - 1 is done with
+		asm volatile("" ::: "memory");
+		if (t + 3 < ntiles) fetch(t + 3);
+		const int64_t row0 = mx4_tile_row(a, split + t * splits);
+		mx4_v16f acc[2];
+		if (!AHEAD) mx4_load_frag<KS, EXACT>(f0, image(t, 0), half, ksteps);
+		if (AHEAD) {
+			mx4_load_frag<KS, EXACT>(f1, image(t, 1), half, ksteps);
+			__builtin_amdgcn_sched_barrier(0);
+		}
+		mx4_shift_scales(f0, half);
+		mx4_tile<KS, EXACT, 2>(f0, w.b, ksteps, acc);
+		mx4_test(w, a, acc, row0, half);
+		if (!AHEAD) mx4_load_frag<KS, EXACT>(f1, image(t, 1), half, ksteps);
+		if (AHEAD && t + 1 < ntiles) {
+			mx4_load_frag<KS, EXACT>(f0, image(t + 1, 0), half, ksteps);
+			__builtin_amdgcn_sched_barrier(0);
+		}
+		mx4_shift_scales(f1, half);
+		mx4_tile<KS, EXACT, 2>(f1, w.b, ksteps, acc);
+		mx4_test(w, a, acc, row0 + 32, half);
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the tile are done before it passes the next barrier
+	}
+	mx4_store_counts(w, a, q0, 2 * split + half, r32);
+}
+
+// The queries that lost keys, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
 // to the best k when the next 128 might not fit.
 template <int KS, bool EXACT>
 __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, const int32_t *over, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
-	__shared__ mx4_key keys[kMx4Cap], best[kMx4ScanMaxK];
+	__shared__ mx4_key keys[kMx4Gather], best[kMx4ScanMaxK];
 	__shared__ int count;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, r32 = lane & 31;
 	for (int q = blockIdx.x; q < a.nq; q += gridDim.x) {
@@ -476,7 +669,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 			}
 			__syncthreads();
 			const int have = count;
-			if (have > kMx4Cap - 128) {
+			if (have > kMx4Gather - 128) {
 				auto key_at = [&](int j) -> mx4_key { return keys[j]; };
 				kth = mx4_block_kth<256>(key_at, have, k, l);
 				if (tid == 0) l.pick = 0;
@@ -499,33 +692,36 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 }
 
 // ---------------------------------------------------------------------------------------------- the plan
-constexpr int kMx4SlabQ = 8192;  // queries whose buffers are held at a time
+constexpr int kMx4SlabQ = 8192;       // queries that are dealt with at a time
+constexpr int kMx4StreamGroups = 4;   // up to so many groups of 64 queries: mx4_stream_kernel, more: mx4_stage_kernel
+constexpr int kMx4StreamWaves = 2048;
 
 struct Mx4Plan {
 	bool chunks;
-	int chunk, parts;  // chunks: rows of one, how many
+	int chunk, parts;  // chunks: rows of one, how many; levels: lists of a query
 	int levels, ratio, first_rows;  // levels after level 0; rows of level 0 (a multiple of 64)
 	int64_t step0;
-	int slab;
+	int slab, qgroups, qtiles, splits;
 	size_t ws;
 };
+
+inline size_t mx4_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
 inline Mx4Plan mx4_plan(int nq, int n, int k)
 {
 	Mx4Plan p{};
-	auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
 	p.chunks = nq <= kMx4ChunkQ;
 	if (p.chunks) {
 		int64_t c = ((int64_t)n + 511) / 512;  // about two workgroups a compute unit
 		c = (c + 127) / 128 * 128;
 		p.chunk = (int)(c < 512 ? 512 : c > kMx4ChunkRows ? kMx4ChunkRows : c);
 		p.parts = (int)(((int64_t)n + p.chunk - 1) / p.chunk);
-		p.ws = up((size_t)nq * p.parts * k * 8 + 8);
+		p.ws = mx4_up((size_t)nq * p.parts * k * 8 + 8);
 		return p;
 	}
 	const int64_t tiles = ((int64_t)n + 63) / 64;
-	// k (ratio - 1) keys are expected of a level: at most a quarter of the buffer
-	const int most = kMx4Cap / 4 / k < 4 ? 4 : kMx4Cap / 4 / k > 10 ? 10 : kMx4Cap / 4 / k;
+	// k (ratio - 1) keys are expected of a level: at most a quarter of what a query can gather
+	const int most = kMx4Gather / 4 / k < 4 ? 4 : kMx4Gather / 4 / k > 10 ? 10 : kMx4Gather / 4 / k;
 	p.levels = 0;
 	p.ratio = 0;
 	p.step0 = 1;
@@ -541,11 +737,38 @@ inline Mx4Plan mx4_plan(int nq, int n, int k)
 	}
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
 	p.slab = nq < kMx4SlabQ ? nq : kMx4SlabQ;
-	p.ws = up((size_t)p.slab * kMx4Cap * 8) + up((size_t)p.slab * 8) + 2 * up((size_t)p.slab * 4) + up((size_t)p.slab * p.first_rows * 4 + 4);
+	p.qgroups = (p.slab + 63) / 64;
+	if (p.qgroups > kMx4StreamGroups) {
+		p.qtiles = (p.qgroups + 7) / 8;
+		p.splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles);  // 8 x qtiles workgroups at a time: one a compute unit
+	} else {
+		const int64_t most_waves = kMx4StreamWaves / p.qgroups;
+		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 1) : most_waves);
+	}
+	p.parts = 2 * p.splits;
+	p.ws = mx4_up((size_t)p.slab * kMx4ScanMaxK * 8) + mx4_up((size_t)p.slab * 8) + 2 * mx4_up((size_t)p.slab * 4) +
+	       mx4_up((size_t)p.slab * p.first_rows * 4 + 4);
+	if (p.levels) p.ws += mx4_up((size_t)p.slab * p.parts * 4) + mx4_up((size_t)p.slab * p.parts * kMx4List * 8);
 	return p;
 }
 
 size_t mx4_scan_workspace(int nq, int n, int k) { return mx4_plan(nq, n, k).ws; }
+
+// once per kernel and device: how much LDS a launch may ask for
+template <int KS, bool EXACT, int WHICH>
+struct Mx4Mark {
+	static inline std::atomic<bool> set[16] = {};
+};
+inline hipError_t mx4_allow_lds(const void *fn, int bytes, std::atomic<bool> (&set)[16])
+{
+	int dev = 0;
+	if (hipGetDevice(&dev) != hipSuccess) return hipErrorInvalidDevice;
+	const bool known = dev >= 0 && dev < 16;
+	if (known && set[dev].load(std::memory_order_relaxed)) return hipSuccess;
+	const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+	if (e == hipSuccess && known) set[dev].store(true, std::memory_order_relaxed);
+	return e;
+}
 
 template <int KS, bool EXACT>
 hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, int k, const uint32_t *allow,
@@ -554,19 +777,11 @@ hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	mx4_key *keys = static_cast<mx4_key *>(ws);
 	const int64_t stride = (int64_t)p.parts * k;
 	const size_t lds = (size_t)nq * p.chunk * 4;
-	static bool set[16] = {};
-	int dev = 0;
-	if (hipGetDevice(&dev) != hipSuccess) return hipErrorInvalidDevice;
-	if (dev < 0 || dev >= 16 || !set[dev]) {
-		const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS, EXACT>), hipFuncAttributeMaxDynamicSharedMemorySize,
-		                                         kMx4ChunkQ * kMx4ChunkRows * 4);
-		if (e != hipSuccess) return e;
-		if (dev >= 0 && dev < 16) set[dev] = true;
-	}
+	const hipError_t e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS, EXACT>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, EXACT, 0>::set);
+	if (e != hipSuccess) return e;
 	if (p.parts > 0)
 		hipLaunchKernelGGL((mx4_chunk_kernel<KS, EXACT>), dim3(p.parts), dim3(256), lds, s, q, nq, rows, n, ksteps, row_bytes, k, p.chunk, allow, keys, stride);
-	hipLaunchKernelGGL((mx4_pick_kernel<1024>), dim3(nq), dim3(1024), 0, s, keys, static_cast<const int32_t *>(nullptr), (int)stride, k, o,
-	                   static_cast<int32_t *>(nullptr));
+	hipLaunchKernelGGL(mx4_pick_chunks_kernel, dim3(nq), dim3(1024), 0, s, keys, (int)stride, k, o);
 	return hipGetLastError();
 }
 
@@ -574,8 +789,18 @@ template <int KS, bool EXACT>
 hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, int k, const uint32_t *allow,
                            const Mx4Out &last, void *ws, hipStream_t s)
 {
-	auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
 	uint8_t *w = static_cast<uint8_t *>(ws);
+	auto take = [&](size_t bytes) -> void * {
+		void *at = w;
+		w += mx4_up(bytes);
+		return at;
+	};
+	mx4_key *best = static_cast<mx4_key *>(take((size_t)p.slab * kMx4ScanMaxK * 8));
+	mx4_key *bound = static_cast<mx4_key *>(take((size_t)p.slab * 8));
+	int32_t *nbest = static_cast<int32_t *>(take((size_t)p.slab * 4));
+	int32_t *over = static_cast<int32_t *>(take((size_t)p.slab * 4));
+	const int m = p.first_rows;
+	float *scores = static_cast<float *>(take((size_t)p.slab * m * 4 + 4));
 	Mx4Level a{};
 	a.q = q;
 	a.rows = rows;
@@ -584,37 +809,35 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	a.n = n;
 	a.ksteps = ksteps;
 	a.row_bytes = row_bytes;
-	a.keys = reinterpret_cast<mx4_key *>(w);
-	w += up((size_t)p.slab * kMx4Cap * 8);
-	mx4_key *bound = reinterpret_cast<mx4_key *>(w);
-	w += up((size_t)p.slab * 8);
 	a.bound = bound;
-	a.fill = reinterpret_cast<int32_t *>(w);
-	w += up((size_t)p.slab * 4);
-	int32_t *over = reinterpret_cast<int32_t *>(w);
-	w += up((size_t)p.slab * 4);
-	float *scores = reinterpret_cast<float *>(w);
-	const Mx4Out mid = {nullptr, nullptr, nullptr, a.keys, bound, a.fill};
-	const int m = p.first_rows;
-	hipError_t e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, ksteps, row_bytes, scores, m, s);
+	a.parts = p.parts;
+	if (p.levels) {
+		a.counts = static_cast<int32_t *>(take((size_t)p.slab * p.parts * 4));
+		a.lists = static_cast<mx4_key *>(take((size_t)p.slab * p.parts * kMx4List * 8));
+	}
+	const Mx4Out mid = {nullptr, nullptr, nullptr, best, bound, nbest};
+	const bool stage = p.qtiles > 0;
+	const int nwaves = stage ? (p.qgroups + p.qtiles - 1) / p.qtiles : 0;
+	const size_t lds = (size_t)kMx4Ring * mx4_image_slots(row_bytes) * 1024;
+	hipError_t e = hipSuccess;
+	if (p.levels && stage)
+		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS, EXACT>), kMx4Ring * mx4_image_slots(mx4_row_bytes(64 * KS)) * 1024,
+		                  Mx4Mark<KS, EXACT, 1>::set);
+	if (e == hipSuccess) e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, ksteps, row_bytes, scores, m, s);
 	if (e != hipSuccess) return e;
-	hipLaunchKernelGGL(mx4_pick_first_kernel, dim3(nq), dim3(256), 0, s, scores, m, p.step0, n, k, allow, p.levels ? mid : last, (int64_t)kMx4Cap, over);
+	hipLaunchKernelGGL(mx4_pick_first_kernel, dim3(nq), dim3(256), 0, s, scores, m, p.step0, n, k, allow, p.levels ? mid : last, (int64_t)kMx4ScanMaxK, over);
 	const int64_t tiles = ((int64_t)n + 63) / 64;
-	a.ratio = p.ratio;
 	a.step = p.step0;
-	const int qgroups = (nq + 63) / 64;
+	a.skip = p.ratio > 1 ? (unsigned)((((uint64_t)1 << 32) + p.ratio - 2) / (p.ratio - 1)) : 0;
 	for (int l = 1; l <= p.levels; l++) {
 		const int64_t before = (tiles + a.step - 1) / a.step;
 		a.step /= p.ratio;
 		a.tiles = (int)((tiles + a.step - 1) / a.step - before);
-		if (a.tiles > 0) {
-			int64_t waves = 2 * (int64_t)a.tiles * qgroups;
-			if (waves > 2048) waves = 2048;
-			int64_t per = (waves + qgroups - 1) / qgroups;  // waves a query group
-			const int64_t blocks = (per * qgroups + 3) / 4;
-			hipLaunchKernelGGL((mx4_stream_kernel<KS, EXACT>), dim3((unsigned)blocks), dim3(256), 0, s, a, qgroups);
-		}
-		hipLaunchKernelGGL((mx4_pick_kernel<256>), dim3(nq), dim3(256), 0, s, a.keys, a.fill, kMx4Cap, k, l < p.levels ? mid : last, over);
+		if (stage)
+			hipLaunchKernelGGL((mx4_stage_kernel<KS, EXACT>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
+		else
+			hipLaunchKernelGGL((mx4_stream_kernel<KS, EXACT>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
+		hipLaunchKernelGGL(mx4_pick_kernel, dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, k, l < p.levels ? mid : last, over);
 	}
 	if (p.levels)
 		hipLaunchKernelGGL((mx4_rescue_kernel<KS, EXACT>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
