@@ -100,39 +100,49 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void *x, int64_
 	if (2 * part < pad) *reinterpret_cast<uint16_t *>(tail + nb + 2 * part) = 0;
 }
 
-// One thread per 8 components
+// One thread per 4 components, kMx4ExpandRun times 256 threads apart: a store writes 16 neighbouring bytes a lane, 1 KB a wave.  Bound by the
+// writing of the values.
+constexpr int kMx4ExpandRun = 4;
+
 __global__ __launch_bounds__(256) void mx4_expand_kernel(const uint8_t *packed, int64_t rows, int dim, int nb, int row_bytes, float *values)
 {
-	const int per_row = 4 * nb;
-	const int64_t first = (int64_t)blockIdx.x * 256;
+	const int per_row = (dim + 3) / 4;
+	const int64_t first = (int64_t)blockIdx.x * (256 * kMx4ExpandRun);
 	const int64_t row0 = first / per_row;
-	const int u = (int)(first - row0 * per_row) + (int)threadIdx.x;
-	const int dr = u / per_row, part = u - dr * per_row;
-	const int64_t row = row0 + dr;
-	const int col = part * 8;
-	if (row >= rows || col >= dim) return;
-	const uint8_t *in = packed + row * row_bytes;
-	const unsigned codes = *reinterpret_cast<const unsigned *>(in + part * 4);
-	const int s = in[16 * nb + (part >> 2)];
-	const float scale = s == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(s > 0 ? (unsigned)s << 23 : 0x00400000u);
-	float f[8];
+	const int u0 = (int)(first - row0 * per_row) + (int)threadIdx.x;
+	unsigned codes[kMx4ExpandRun];
+	int s[kMx4ExpandRun];
+	int64_t at[kMx4ExpandRun];
+	int left[kMx4ExpandRun];
 #pragma unroll
-	for (int i = 0; i < 8; i++) {
-		const unsigned c = (codes >> (4 * i)) & 15u, ex = (c >> 1) & 3u, m = c & 1u;
-		// 2^(ex - 1) (1 + m / 2), or m / 2 where ex = 0
-		const float mag = ex ? __uint_as_float(((ex + 126u) << 23) | (m << 22)) : 0.5f * (float)m;
-		f[i] = ((c & 8u) ? -mag : mag) * scale;
+	for (int j = 0; j < kMx4ExpandRun; j++) {
+		const int u = u0 + 256 * j, dr = u / per_row, part = u - dr * per_row;
+		const int64_t row = row0 + dr;
+		left[j] = row < rows ? dim - part * 4 : 0;
+		const uint8_t *in = packed + (row < rows ? row : 0) * row_bytes;
+		codes[j] = *reinterpret_cast<const uint16_t *>(in + part * 2);
+		s[j] = in[16 * nb + (part >> 3)];
+		at[j] = row * dim + part * 4;
 	}
-	float *out = values + row * dim + col;
-	if (col + 8 <= dim) {
-		Mx4Float8 t;
 #pragma unroll
-		for (int i = 0; i < 8; i++) t.v[i] = f[i];
-		*reinterpret_cast<Mx4Float8 *>(out) = t;
-	} else {
+	for (int j = 0; j < kMx4ExpandRun; j++) {
+		if (left[j] <= 0) continue;
+		const float scale = s[j] == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(s[j] > 0 ? (unsigned)s[j] << 23 : 0x00400000u);
+		Mx4Float4 t;
 #pragma unroll
-		for (int i = 0; i < 8; i++)
-			if (col + i < dim) out[i] = f[i];
+		for (int i = 0; i < 4; i++) {
+			const unsigned c = (codes[j] >> (4 * i)) & 15u, ex = (c >> 1) & 3u, m = c & 1u;
+			// 2^(ex - 1) (1 + m / 2), or m / 2 where ex = 0
+			const float mag = ex ? __uint_as_float(((ex + 126u) << 23) | (m << 22)) : 0.5f * (float)m;
+			t.v[i] = ((c & 8u) ? -mag : mag) * scale;
+		}
+		if (left[j] >= 4) {
+			*reinterpret_cast<Mx4Float4 *>(values + at[j]) = t;
+		} else {
+#pragma unroll
+			for (int i = 0; i < 3; i++)
+				if (i < left[j]) values[at[j] + i] = t.v[i];
+		}
 	}
 }
 
@@ -163,7 +173,8 @@ hipError_t mx4_launch_expand(const uint8_t *packed, int64_t rows, int dim, float
 	const int64_t step = (int64_t)1 << 22;
 	for (int64_t r = 0; r < rows; r += step) {
 		const int64_t m = rows - r < step ? rows - r : step;
-		hipLaunchKernelGGL(mx4_expand_kernel, dim3((unsigned)mx4_row_groups(m, dim)), dim3(256), 0, s, packed + r * rb, m, dim, nb, rb,
+		const int64_t groups = (m * ((dim + 3) / 4) + 256 * kMx4ExpandRun - 1) / (256 * kMx4ExpandRun);
+		hipLaunchKernelGGL(mx4_expand_kernel, dim3((unsigned)groups), dim3(256), 0, s, packed + r * rb, m, dim, nb, rb,
 		                   values + r * dim);
 	}
 	return hipGetLastError();

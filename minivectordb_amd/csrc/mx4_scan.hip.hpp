@@ -253,34 +253,7 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 	mx4_block_topk<256>(key_at, m, k, q, kMx4ScanMaxK, o, l, best);
 }
 
-// ---------------------------------------------------------------------------------------------- queries in registers
-// The fragments of 32 queries (columns of D) for KS steps of 64 components, and their scale bytes: pieces 2 s + half of step s.  KS is
-// at least the row's number of steps; what is past it stays 0.
-template <int KS>
-struct Mx4Frag {
-	mx4_v4i d[KS];
-	int sc[(KS + 1) / 2];  // byte 0: the scale of an even step, byte 2: of the odd one after it
-};
-
-// exact: KS is the row's number of steps
-template <int KS, bool EXACT>
-__device__ __forceinline__ void mx4_load_frag(Mx4Frag<KS> &f, const uint8_t *row, int half, int ksteps)
-{
-#pragma unroll
-	for (int s = 0; s < KS; s++)
-		if (EXACT || s < ksteps) f.d[s] = *reinterpret_cast<const mx4_v4i *>(row + (2 * s + half) * 16);
-	const int *sp = reinterpret_cast<const int *>(row + 32 * (EXACT ? KS : ksteps));
-#pragma unroll
-	for (int s = 0; s < (KS + 1) / 2; s++)
-		if (EXACT || 2 * s < ksteps) f.sc[s] = sp[s];
-}
-template <int KS>
-__device__ __forceinline__ void mx4_shift_scales(Mx4Frag<KS> &f, int half)
-{
-#pragma unroll
-	for (int s = 0; s < (KS + 1) / 2; s++) f.sc[s] = (int)((unsigned)f.sc[s] >> (8 * half));
-}
-
+// ---------------------------------------------------------------------------------------------- products of 32 rows
 // acc[c] = the products of the 32 rows in `a` (rows of D) with the 32 queries in b[c]
 template <int KS, bool EXACT, int C>
 __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS> (&b)[C], int ksteps, mx4_v16f (&acc)[C])
@@ -863,22 +836,7 @@ hipError_t mx4_launch_scan(const uint8_t *q, int nq, const uint8_t *rows, int n,
 			e = p.chunks ? mx4_scan_chunks<KS, EXACT>(p, q + q0 * rb, m, rows, n, ks, rb, k, allow, o, ws, s)
 			             : mx4_scan_levels<KS, EXACT>(p, q + q0 * rb, m, rows, n, ks, rb, k, allow, o, ws, s);
 		};
-		using std::integral_constant;
-		switch (ks) {
-		case 1: go(integral_constant<int, 1>{}, std::true_type{}); break;
-		case 2: go(integral_constant<int, 2>{}, std::true_type{}); break;
-		case 3: go(integral_constant<int, 3>{}, std::true_type{}); break;
-		case 4: go(integral_constant<int, 4>{}, std::true_type{}); break;
-		case 5: go(integral_constant<int, 5>{}, std::true_type{}); break;
-		case 6: go(integral_constant<int, 6>{}, std::true_type{}); break;
-		case 7: go(integral_constant<int, 7>{}, std::true_type{}); break;
-		case 8: go(integral_constant<int, 8>{}, std::true_type{}); break;
-		case 9: case 10: case 11: go(integral_constant<int, 12>{}, std::false_type{}); break;
-		case 12: go(integral_constant<int, 12>{}, std::true_type{}); break;
-		case 13: case 14: case 15: go(integral_constant<int, 16>{}, std::false_type{}); break;
-		case 16: go(integral_constant<int, 16>{}, std::true_type{}); break;
-		default: break;
-		}
+		mx4_for_steps(ks, go);
 		if (e != hipSuccess) return e;
 	}
 	return hipSuccess;
