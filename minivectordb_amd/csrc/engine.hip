@@ -1913,8 +1913,7 @@ int mvdb_mx4_product_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_
 
 size_t mvdb_mx4_scan_workspace(const mvdb_index *h, int nq, int n, int k)
 {
-	(void)h;
-	return nq > 0 && n >= 0 && k > 0 && k <= kMx4ScanMaxK ? mx4_scan_workspace(nq, n, k) : 0;
+	return nq > 0 && n >= 0 && k > 0 && k <= kMx4ScanMaxK && h->cfg.dim <= kMx4ScanMaxDim ? mx4_scan_workspace(nq, n, h->cfg.dim, k) : 0;
 }
 
 int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, int k, const uint32_t *d_allow,
@@ -1928,7 +1927,7 @@ int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint
 	if (!d_q || (n > 0 && !d_rows) || !d_out_ids || !d_out_val || !d_out_count || !d_ws) return mx4_fail(h, fn, "null pointer");
 	if (mx4_misaligned(d_q) || mx4_misaligned(d_rows)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
 	if (mx4_misaligned(d_ws)) return mx4_fail(h, fn, "the workspace must be 16-byte aligned");
-	if (ws_bytes < mx4_scan_workspace(nq, n, k)) return mx4_fail(h, fn, "the workspace is smaller than mvdb_mx4_scan_workspace says");
+	if (ws_bytes < mx4_scan_workspace(nq, n, h->cfg.dim, k)) return mx4_fail(h, fn, "the workspace is smaller than mvdb_mx4_scan_workspace says");
 	DeviceGuard dev(h);
 	if (!dev.ok) return 0;
 	hipStream_t s = static_cast<hipStream_t>(stream);
@@ -2056,7 +2055,7 @@ int mvdb_mx4_scan_many(mvdb_index *h, const float *q, int nq, int k, const uint3
 		if (!d_allow) return mx4_fail(h, fn, "out of device memory (staging)");
 		HIP_OK(h, hipMemcpy(d_allow, allow, bytes, hipMemcpyHostToDevice));
 	}
-	const size_t ws = mx4_scan_workspace(nq, n, k), cells = (size_t)nq * k * 4;
+	const size_t ws = mx4_scan_workspace(nq, n, h->cfg.dim, k), cells = (size_t)nq * k * 4;
 	int32_t *d_ids = static_cast<int32_t *>(h->st_ids.need(cells));
 	float *d_val = static_cast<float *>(h->st_dist.need(cells));
 	int32_t *d_cnt = static_cast<int32_t *>(h->st_cnt.need((size_t)nq * 4));

@@ -25,15 +25,15 @@ constexpr int kMx4MaxDim = 4096;      // quantise, expand, product
 constexpr int kMx4ScanMaxDim = 1024;  // scan (as the traversal)
 constexpr int kMx4ScanMaxK = 128;
 
-__host__ __device__ inline int mx4_blocks(int dim) { return 2 * ((dim + 63) / 64); }
-__host__ __device__ inline int mx4_row_bytes(int dim) { return 16 * mx4_blocks(dim) + (mx4_blocks(dim) + 15) / 16 * 16; }
+__host__ __device__ constexpr int mx4_blocks(int dim) { return 2 * ((dim + 63) / 64); }
+__host__ __device__ constexpr int mx4_row_bytes(int dim) { return 16 * mx4_blocks(dim) + (mx4_blocks(dim) + 15) / 16 * 16; }
 
 // dtype of the rows that are quantised: 0 f32, 1 bf16, 2 f16; ld = components from one row to the next
 hipError_t mx4_launch_quantize(const void *x, int dtype, int64_t rows, int dim, int64_t ld, uint8_t *packed, hipStream_t s);
 hipError_t mx4_launch_expand(const uint8_t *packed, int64_t rows, int dim, float *values, hipStream_t s);
 // out[q][r], ldo floats from one query to the next
 hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, float *out, int64_t ldo, hipStream_t s);
-size_t mx4_scan_workspace(int nq, int n, int k);
+size_t mx4_scan_workspace(int nq, int n, int dim, int k);
 // ws: mx4_scan_workspace bytes, 16-byte aligned, used by this call until it has run on the stream
 hipError_t mx4_launch_scan(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, int k, const uint32_t *allow, int32_t *out_ids,
                            float *out_val, int32_t *out_count, void *ws, hipStream_t s);

@@ -24,25 +24,23 @@ __device__ __forceinline__ mx4_v16f mx4_mfma(const mx4_v4i &a, int sa, const mx4
 	return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, OA, sa, OB, sb);
 }
 
-// The fragments of 32 packed rows for KS steps of 64 components, and their scale bytes: pieces 2 s + half of step s.  KS is at least the
-// row's number of steps; steps past it are never touched.
+// The fragments of 32 packed rows of KS steps of 64 components, and their scale bytes: pieces 2 s + half of step s
 template <int KS>
 struct Mx4Frag {
 	mx4_v4i d[KS];
 	int sc[(KS + 1) / 2];  // byte 0: the scale of an even step, byte 2: of the odd one after it
 };
 
-// exact: KS is the row's number of steps
-template <int KS, bool EXACT>
-__device__ __forceinline__ void mx4_load_frag(Mx4Frag<KS> &f, const uint8_t *row, int half, int ksteps)
+template <int KS>
+__device__ __forceinline__ void mx4_load_frag(Mx4Frag<KS> &f, const uint8_t *row, int half)
 {
 #pragma unroll
 	for (int s = 0; s < KS; s++)
-		if (EXACT || s < ksteps) f.d[s] = *reinterpret_cast<const mx4_v4i *>(row + (2 * s + half) * 16);
-	const int *sp = reinterpret_cast<const int *>(row + 32 * (EXACT ? KS : ksteps));
+		f.d[s] = *reinterpret_cast<const mx4_v4i *>(row + (2 * s + half) * 16);
+	const int *sp = reinterpret_cast<const int *>(row + 32 * KS);
 #pragma unroll
 	for (int s = 0; s < (KS + 1) / 2; s++)
-		if (EXACT || 2 * s < ksteps) f.sc[s] = sp[s];
+		f.sc[s] = sp[s];
 }
 template <int KS>
 __device__ __forceinline__ void mx4_shift_scales(Mx4Frag<KS> &f, int half)
@@ -51,87 +49,80 @@ __device__ __forceinline__ void mx4_shift_scales(Mx4Frag<KS> &f, int half)
 	for (int s = 0; s < (KS + 1) / 2; s++) f.sc[s] = (int)((unsigned)f.sc[s] >> (8 * half));
 }
 
-// go(KS, EXACT) for a row of `ks` steps, 1 .. 16: kernels are there for 1 .. 8, 12 and 16 steps
-template <typename F>
+// go(KS) for a row of `ks` steps, 1 .. 16
+template <int KS = 1, typename F>
 inline void mx4_for_steps(int ks, F go)
 {
-	using std::integral_constant;
-	switch (ks) {
-	case 1: go(integral_constant<int, 1>{}, std::true_type{}); break;
-	case 2: go(integral_constant<int, 2>{}, std::true_type{}); break;
-	case 3: go(integral_constant<int, 3>{}, std::true_type{}); break;
-	case 4: go(integral_constant<int, 4>{}, std::true_type{}); break;
-	case 5: go(integral_constant<int, 5>{}, std::true_type{}); break;
-	case 6: go(integral_constant<int, 6>{}, std::true_type{}); break;
-	case 7: go(integral_constant<int, 7>{}, std::true_type{}); break;
-	case 8: go(integral_constant<int, 8>{}, std::true_type{}); break;
-	case 9: case 10: case 11: go(integral_constant<int, 12>{}, std::false_type{}); break;
-	case 12: go(integral_constant<int, 12>{}, std::true_type{}); break;
-	case 13: case 14: case 15: go(integral_constant<int, 16>{}, std::false_type{}); break;
-	case 16: go(integral_constant<int, 16>{}, std::true_type{}); break;
-	default: break;
-	}
+	if (ks == KS)
+		go(std::integral_constant<int, KS>{});
+	else if constexpr (KS < 16)
+		mx4_for_steps<KS + 1>(ks, go);
 }
 
 struct Mx4Product {
 	const uint8_t *q, *rows;
-	int nq, n, ksteps, row_bytes;
+	int nq, n;
 	float *out;
 	int64_t ldo;
-	int groups, cols, run;  // groups of 64 queries; columns; steps of 128 columns a workgroup
+	int groups, cols, run;  // groups of 32 * mx4_product_frags queries; columns; steps of 128 columns a workgroup
+	int block;              // chunks of an XCD that are gone through for one group of queries after the other
 	int64_t step;
 };
+
+// fragments of 32 queries a wave holds: as many as leave room in its registers for the rows
+__host__ __device__ constexpr int mx4_product_frags(int ks) { return ks <= 8 ? 2 : 1; }
 
 // Column c of the result is row c, or (step > 1) row 64 * step * (c / 64) + c % 64: the 64-row tiles that are multiples of step.  Columns past the
 // last row hold products that nobody reads.
 //
-// Bound by the writing of the result (4 bytes for every 2 * dim operations).  A wave holds 64 queries in registers and takes 32 rows at a time, the
+// Bound by the writing of the result (4 bytes for every 2 * dim operations).  A wave holds 64 queries (32 where rows are long) in registers and takes 32 rows at a time, the
 // next ones on their way meanwhile; the four waves of a workgroup take neighbouring rows, so that together they write 512 bytes of each of 64
-// result rows.  Queries are the rows of D, so a store writes 128 bytes of two result rows.  Workgroups that follow each other on one XCD take
-// the same rows for other queries: those come from that XCD's L2.
-template <int KS, bool EXACT, bool STREAM>
+// result rows.  Queries are the rows of D, so a store writes 128 bytes of two result rows.  The workgroups of one XCD go through a block of
+// rows that stays in its L2, one group of queries after the other: what is written at a time lies side by side in a result row rather than at
+// one place of many rows, which a power of two as the row length would put into the same memory channels.
+template <int KS, bool STREAM>
 __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 {
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
-	const int j8 = blockIdx.x >> 3, group = j8 % a.groups;
-	const int64_t chunk = (int64_t)(j8 / a.groups) * 8 + (blockIdx.x & 7);
-	const int row_bytes = EXACT ? 32 * KS + (2 * KS + 15) / 16 * 16 : a.row_bytes, ksteps = EXACT ? KS : a.ksteps;
+	const int j8 = blockIdx.x >> 3, j = j8 % (a.groups * a.block);
+	const int group = j / a.block;
+	const int64_t chunk = ((int64_t)(j8 / (a.groups * a.block)) * a.block + j % a.block) * 8 + (blockIdx.x & 7);
+	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	int64_t col0 = chunk * a.run * 128 + wave * 32;
 	if (col0 >= a.cols) return;
-	const int q0 = group * 64;
-	Mx4Frag<KS> qf[2];
+	constexpr int C = mx4_product_frags(KS);
+	const int q0 = group * 32 * C;
+	Mx4Frag<KS> qf[C];
 #pragma unroll
-	for (int c = 0; c < 2; c++) {
+	for (int c = 0; c < C; c++) {
 		const int q = q0 + c * 32 + r32;
-		mx4_load_frag<KS, EXACT>(qf[c], a.q + (int64_t)(q < a.nq ? q : a.nq - 1) * row_bytes, half, ksteps);
-		mx4_shift_scales(qf[c], half);
+		mx4_load_frag<KS>(qf[c], a.q + (int64_t)(q < a.nq ? q : a.nq - 1) * row_bytes, half);
 	}
 	const int64_t end = (chunk + 1) * a.run * 128 < a.cols ? (chunk + 1) * a.run * 128 : a.cols;
 	auto load = [&](int64_t col, Mx4Frag<KS> &f) {
 		const int64_t at = (col & ~(int64_t)63) * a.step + (col & 63) + r32;
-		mx4_load_frag<KS, EXACT>(f, a.rows + (at < a.n ? at : a.n - 1) * row_bytes, half, ksteps);
+		mx4_load_frag<KS>(f, a.rows + (at < a.n ? at : a.n - 1) * row_bytes, half);
 	};
 	auto use = [&](int64_t col, Mx4Frag<KS> &f) {
 		mx4_shift_scales(f, half);
-		mx4_v16f acc[2];
+		mx4_v16f acc[C];
 		const mx4_v16f zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-		for (int s = 0; s < KS; s++)
-			if (EXACT || s < ksteps) {
+		for (int s = 0; s < KS; s++) {
 #pragma unroll
-				for (int c = 0; c < 2; c++) {
+				for (int c = 0; c < C; c++) {
 					const mx4_v16f &in = s == 0 ? zero : acc[c];
 					acc[c] = (s & 1) ? mx4_mfma<2, 2>(qf[c].d[s], qf[c].sc[s / 2], f.d[s], f.sc[s / 2], in)
 					                 : mx4_mfma<0, 0>(qf[c].d[s], qf[c].sc[s / 2], f.d[s], f.sc[s / 2], in);
 				}
 			}
 #pragma unroll
-		for (int c = 0; c < 2; c++) asm volatile("" : "+v"(acc[c]));  // see mx4_tile
-		const bool full = q0 + 64 <= a.nq && col + 32 <= a.cols;
+		for (int c = 0; c < C; c++) asm volatile("" : "+v"(acc[c]));  // see mx4_tile
+		const bool full = q0 + 32 * C <= a.nq && col + 32 <= a.cols;
 		float *o = a.out + (q0 + 4 * half) * a.ldo + col + r32;
 		if (full) {
 #pragma unroll
-			for (int c = 0; c < 2; c++)
+			for (int c = 0; c < C; c++)
 #pragma unroll
 				for (int i = 0; i < 16; i++) {
 					float *p = o + (c * 32 + 8 * (i >> 2) + (i & 3)) * a.ldo;
@@ -142,7 +133,7 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 				}
 		} else if (col + r32 < a.cols) {
 #pragma unroll
-			for (int c = 0; c < 2; c++)
+			for (int c = 0; c < C; c++)
 #pragma unroll
 				for (int i = 0; i < 16; i++) {
 					const int q = c * 32 + 8 * (i >> 2) + (i & 3);
@@ -150,9 +141,16 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 				}
 		}
 	};
+	// the first rows are asked for before the queries are waited for
+	auto ready = [&]() {
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int c = 0; c < C; c++) mx4_shift_scales(qf[c], half);
+	};
 	if constexpr (KS <= 8) {
 		Mx4Frag<KS> f0, f1;
 		load(col0, f0);
+		ready();
 		while (true) {
 			if (col0 + 128 < end) load(col0 + 128, f1);
 			__builtin_amdgcn_sched_barrier(0);
@@ -166,10 +164,14 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 			if (col0 >= end) break;
 		}
 	} else {
-		for (; col0 < end; col0 += 128) {
-			Mx4Frag<KS> f;
-			load(col0, f);
+		Mx4Frag<KS> f;
+		load(col0, f);
+		ready();
+		while (true) {
 			use(col0, f);
+			col0 += 128;
+			if (col0 >= end) break;
+			load(col0, f);
 		}
 	}
 }
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(256) void mx4_product_long_kernel(const uint8_t *q,
 
 constexpr int kMx4ProductQ = 4096;       // queries a launch
 constexpr int kMx4ProductGroups = 4096;  // workgroups a launch, about
+constexpr int64_t kMx4BlockBytes = 4 << 20;  // rows of a block: an XCD's L2
 constexpr int64_t kMx4StreamBytes = 256 << 20;  // results that are larger than the caches go past them
 
 // `cols` columns
@@ -241,8 +244,6 @@ inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8
 		a.q = q;
 		a.rows = rows;
 		a.n = n;
-		a.ksteps = ksteps;
-		a.row_bytes = row_bytes;
 		a.ldo = ldo;
 		a.cols = cols;
 		a.step = step;
@@ -251,19 +252,23 @@ inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8
 			a.nq = (int)(nq - q0 < kMx4ProductQ ? nq - q0 : kMx4ProductQ);
 			a.q = q + q0 * row_bytes;
 			a.out = out + q0 * ldo;
-			a.groups = (a.nq + 63) / 64;
+			const int frags = mx4_product_frags(ksteps);
+			a.groups = (a.nq + 32 * frags - 1) / (32 * frags);
 			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries; but all of a small result's at once
 			int64_t run = rtiles * a.groups / kMx4ProductGroups;
 			a.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
 			const int64_t chunks = (rtiles + a.run - 1) / a.run;
-			const int64_t blocks = (chunks + 7) / 8 * 8 * a.groups;
-			mx4_for_steps(ksteps, [&](auto steps, auto exact) {
+			const int64_t per_xcd = (chunks + 7) / 8, fit = kMx4BlockBytes / ((int64_t)a.run * 128 * row_bytes);
+			// With up to 16 groups the workgroups in flight spread over enough columns by themselves and share each row at once (1000 x 262 144 x
+			// 384: block 1 189 us, blocks of an L2 199); with 64 they do not (4096 x 65 536 x 512: 254 and 214).
+			a.block = (int)(a.groups <= 16 || fit < 1 ? 1 : fit < per_xcd ? fit : per_xcd);
+			const int64_t blocks = (per_xcd + a.block - 1) / a.block * a.block * 8 * a.groups;
+			mx4_for_steps(ksteps, [&](auto steps) {
 				constexpr int KS = decltype(steps)::value;
-				constexpr bool EXACT = decltype(exact)::value;
-				if (stream)
-					hipLaunchKernelGGL((mx4_product_kernel<KS, EXACT, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+					if (stream)
+					hipLaunchKernelGGL((mx4_product_kernel<KS, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
 				else
-					hipLaunchKernelGGL((mx4_product_kernel<KS, EXACT, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+					hipLaunchKernelGGL((mx4_product_kernel<KS, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
 			});
 		}
 		return hipGetLastError();

@@ -255,13 +255,12 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 
 // ---------------------------------------------------------------------------------------------- products of 32 rows
 // acc[c] = the products of the 32 rows in `a` (rows of D) with the 32 queries in b[c]
-template <int KS, bool EXACT, int C>
-__device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS> (&b)[C], int ksteps, mx4_v16f (&acc)[C])
+template <int KS, int C>
+__device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS> (&b)[C], mx4_v16f (&acc)[C])
 {
 	const mx4_v16f zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-	for (int s = 0; s < KS; s++)
-		if (EXACT || s < ksteps) {
+	for (int s = 0; s < KS; s++) {
 #pragma unroll
 			for (int c = 0; c < C; c++) {
 				const mx4_v16f &in = s == 0 ? zero : acc[c];
@@ -280,35 +279,61 @@ __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS>
 constexpr int kMx4ChunkQ = 8;        // queries a launch, at most
 constexpr int kMx4ChunkRows = 2048;  // rows a workgroup, at most
 
-// A workgroup = 4 waves; a wave takes 32 rows at a time.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
+constexpr int kMx4ChunkThreads = 512;
+
+// A wave takes 32 rows at a time, the next ones on their way meanwhile.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
 // quarters of the matrix work is for nothing: it is a few us at a million rows, against the reading of them.
-template <int KS, bool EXACT>
-__global__ __launch_bounds__(256) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, int k, int chunk,
-                                                        const uint32_t *allow, mx4_key *out, int64_t stride)
+template <int KS>
+__global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int k, int chunk,
+                                                                     const uint32_t *allow, mx4_key *out, int64_t stride)
 {
 	extern __shared__ float sc[];  // [nq][chunk]
 	__shared__ Mx4PickLds l;
-	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, r32 = lane & 31;
-	Mx4Frag<KS> b[1];
-	mx4_load_frag<KS, EXACT>(b[0], q + (int64_t)(r32 < nq ? r32 : nq - 1) * row_bytes, half, ksteps);
-	mx4_shift_scales(b[0], half);
+	constexpr int row_bytes = mx4_row_bytes(64 * KS);
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, r32 = lane & 31;
 	const int64_t first = (int64_t)blockIdx.x * chunk;
 	const int m = (int)(n - first < chunk ? n - first : chunk);
 	const uint8_t *base = rows + first * row_bytes;
-	for (int t = wave * 32; t < m; t += 128) {
+	Mx4Frag<KS> b[1], f0, f1;
+	auto load = [&](int t, Mx4Frag<KS> &f) {
 		const int r = t + r32 < m ? t + r32 : m - 1;
-		Mx4Frag<KS> a;
-		mx4_load_frag<KS, EXACT>(a, base + (int64_t)r * row_bytes, half, ksteps);
-		mx4_shift_scales(a, half);
+		mx4_load_frag<KS>(f, base + (int64_t)r * row_bytes, half);
+	};
+	auto use = [&](int t, Mx4Frag<KS> &f) {
+		mx4_shift_scales(f, half);
 		mx4_v16f acc[1];
-		mx4_tile<KS, EXACT, 1>(a, b, ksteps, acc);
+		mx4_tile<KS, 1>(f, b, acc);
 		if (r32 < nq) {
 #pragma unroll
-			for (int i = 0; i < 16; i++) {
-				const int at = t + 8 * (i >> 2) + 4 * half + (i & 3);
-				if (at < m) sc[r32 * chunk + at] = acc[0][i];
+			for (int g = 0; g < 4; g++) {
+				const int at = t + 8 * g + 4 * half;
+				float *o = sc + r32 * chunk + at;  // (chunk is a multiple of 4)
+				if (at + 4 <= m) {
+					*reinterpret_cast<float4 *>(o) = make_float4(acc[0][4 * g], acc[0][4 * g + 1], acc[0][4 * g + 2], acc[0][4 * g + 3]);
+				} else {
+#pragma unroll
+					for (int j = 0; j < 3; j++)
+						if (at + j < m) o[j] = acc[0][4 * g + j];
+				}
 			}
 		}
+	};
+	constexpr int STEP = kMx4ChunkThreads / 2;  // 32 rows a wave
+	int t = wave * 32;
+	mx4_load_frag<KS>(b[0], q + (int64_t)(r32 < nq ? r32 : nq - 1) * row_bytes, half);
+	if (t < m) load(t, f0);
+	__builtin_amdgcn_sched_barrier(0);
+	mx4_shift_scales(b[0], half);
+	while (t < m) {
+		if (t + STEP < m) load(t + STEP, f1);
+		__builtin_amdgcn_sched_barrier(0);
+		use(t, f0);
+		t += STEP;
+		if (t >= m) break;
+		if (t + STEP < m) load(t + STEP, f0);
+		__builtin_amdgcn_sched_barrier(0);
+		use(t, f1);
+		t += STEP;
 	}
 	__syncthreads();
 	for (int qi = 0; qi < nq; qi++) {
@@ -317,17 +342,17 @@ __global__ __launch_bounds__(256) void mx4_chunk_kernel(const uint8_t *q, int nq
 			if (allow && !((allow[id >> 5] >> (id & 31)) & 1u)) return 0;
 			return mx4_make_key(sc[qi * chunk + j], (unsigned)id);
 		};
-		const mx4_key kth = mx4_block_kth<256>(key_at, m, k, l);
+		const mx4_key kth = mx4_block_kth<kMx4ChunkThreads>(key_at, m, k, l);
 		mx4_key *o = out + qi * stride + (int64_t)blockIdx.x * k;
 		if (tid == 0) l.pick = 0;
 		__syncthreads();
-		for (int j = tid; j < m; j += 256) {
+		for (int j = tid; j < m; j += kMx4ChunkThreads) {
 			const mx4_key key = key_at(j);
 			if (key >= kth) o[atomicAdd(&l.pick, 1)] = key;
 		}
 		__syncthreads();
 		const int have = l.pick;
-		for (int j = have + tid; j < k; j += 256) o[j] = 0;
+		for (int j = have + tid; j < k; j += kMx4ChunkThreads) o[j] = 0;
 		__syncthreads();
 	}
 }
@@ -338,7 +363,7 @@ constexpr int kMx4FirstTiles = 16;  // 64-row tiles of level 0, at most
 struct Mx4Level {
 	const uint8_t *q, *rows;
 	const uint32_t *allow;
-	int nq, n, ksteps, row_bytes;
+	int nq, n;
 	int64_t step;     // see mx4_level_tile
 	unsigned skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
 	int tiles;
@@ -362,23 +387,23 @@ __device__ __forceinline__ uint32_t mx4_allow_word(const uint32_t *allow, int64_
 	return ((const_ptr_t)(allow))[at];
 }
 
-// 64 queries of a wave: two fragments of 32, and for each this lane's query, its bound and its list
-template <int KS>
+// Queries of a wave: C fragments of 32, and for each this lane's query, its bound and its list
+template <int KS, int C>
 struct Mx4Queries {
-	Mx4Frag<KS> b[2];
-	float bound[2];
-	mx4_key bkey[2];
-	unsigned list[2];  // index of the list's first key
-	int count[2];
+	Mx4Frag<KS> b[C];
+	float bound[C];
+	mx4_key bkey[C];
+	unsigned list[C];  // index of the list's first key
+	int count[C];
 };
 
-template <int KS, bool EXACT>
-__device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS> &w, const Mx4Level &a, int q0, int part, int half, int r32, int ksteps, int row_bytes)
+template <int KS, int C>
+__device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS, C> &w, const Mx4Level &a, int q0, int part, int half, int r32)
 {
 #pragma unroll
-	for (int c = 0; c < 2; c++) {
+	for (int c = 0; c < C; c++) {
 		const int q = q0 + c * 32 + r32, qs = q < a.nq ? q : a.nq - 1;
-		mx4_load_frag<KS, EXACT>(w.b[c], a.q + (int64_t)qs * row_bytes, half, ksteps);
+		mx4_load_frag<KS>(w.b[c], a.q + (int64_t)qs * mx4_row_bytes(64 * KS), half);
 		mx4_shift_scales(w.b[c], half);
 		w.bkey[c] = a.bound[qs];
 		// no query in this column: nothing is >= NaN
@@ -387,21 +412,21 @@ __device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS> &w, const Mx4Lev
 		w.count[c] = 0;
 	}
 }
-template <int KS>
-__device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS> &w, const Mx4Level &a, int q0, int part, int r32)
+template <int KS, int C>
+__device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS, C> &w, const Mx4Level &a, int q0, int part, int r32)
 {
 #pragma unroll
-	for (int c = 0; c < 2; c++)
+	for (int c = 0; c < C; c++)
 		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = w.count[c];
 }
 
 // Products of 32 rows (row0 ..) with the wave's queries: test, and append what passes.  The test is one maximum over the lane's 16 rows; who
 // passed is looked for four rows at a time.
-template <int KS>
-__device__ __forceinline__ void mx4_test(Mx4Queries<KS> &w, const Mx4Level &a, const mx4_v16f (&acc)[2], int64_t row0, int half)
+template <int KS, int C>
+__device__ __forceinline__ void mx4_test(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], int64_t row0, int half)
 {
 #pragma unroll
-	for (int c = 0; c < 2; c++) {
+	for (int c = 0; c < C; c++) {
 		float m[4];
 #pragma unroll
 		for (int g = 0; g < 4; g++) m[g] = __builtin_fmaxf(__builtin_fmaxf(acc[c][4 * g], acc[c][4 * g + 1]), __builtin_fmaxf(acc[c][4 * g + 2], acc[c][4 * g + 3]));
@@ -428,17 +453,21 @@ __device__ __forceinline__ void mx4_test(Mx4Queries<KS> &w, const Mx4Level &a, c
 	}
 }
 
-// Independent waves: each holds 64 queries and takes every (waves)-th half tile of the level straight from memory, the next one's rows under
+// fragments of 32 queries a wave of the stream kernel holds
+__host__ __device__ constexpr int mx4_stream_frags(int ks) { return ks <= 8 ? 2 : 1; }
+
+// Independent waves: each holds 64 queries (32 where rows are long) and takes every (waves)-th half tile of the level straight from memory, the next one's rows under
 // way while it multiplies.
-template <int KS, bool EXACT>
+template <int KS>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgroups)
 {
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
 	const int gw = blockIdx.x * 4 + wave, group = gw % qgroups, waves = a.parts / 2, first = gw / qgroups;
 	if (first >= waves) return;
-	const int row_bytes = EXACT ? 32 * KS + (2 * KS + 15) / 16 * 16 : a.row_bytes, ksteps = EXACT ? KS : a.ksteps;
-	Mx4Queries<KS> w;
-	mx4_load_queries<KS, EXACT>(w, a, group * 64, 2 * first + half, half, r32, ksteps, row_bytes);
+	constexpr int row_bytes = mx4_row_bytes(64 * KS);
+	constexpr int C = mx4_stream_frags(KS);
+	Mx4Queries<KS, C> w;
+	mx4_load_queries(w, a, group * 32 * C, 2 * first + half, half, r32);
 	const unsigned total = 2 * (unsigned)a.tiles;
 	// half tile i: its first row and which of its rows count, and (unless none does) the rows
 	auto load = [&](unsigned i, Mx4Frag<KS> &f, int64_t &row0, unsigned &keep) {
@@ -449,7 +478,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 		if (a.allow) keep &= mx4_allow_word(a.allow, row0 >> 5);
 		if (keep == 0) return;
 		const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
-		mx4_load_frag<KS, EXACT>(f, a.rows + r * row_bytes, half, ksteps);
+		mx4_load_frag<KS>(f, a.rows + r * row_bytes, half);
 	};
 	auto use = [&](Mx4Frag<KS> &f, int64_t row0, unsigned keep) {
 		if (keep == 0) return;
@@ -457,11 +486,11 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 #pragma unroll
 		for (int s = 0; s < (KS + 1) / 2; s++) f.sc[s] = out ? -1 : f.sc[s];
 		mx4_shift_scales(f, half);
-		mx4_v16f acc[2];
-		mx4_tile<KS, EXACT, 2>(f, w.b, ksteps, acc);
+		mx4_v16f acc[C];
+		mx4_tile<KS, C>(f, w.b, acc);
 		mx4_test(w, a, acc, row0, half);
 	};
-	if constexpr (KS <= 8) {
+	if constexpr (KS <= 12) {
 		Mx4Frag<KS> f0, f1;
 		int64_t row0, row1;
 		unsigned keep0 = 0, keep1 = 0;
@@ -489,7 +518,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 			use(f, row0, keep);
 		}
 	}
-	mx4_store_counts(w, a, group * 64, 2 * first + half, r32);
+	mx4_store_counts(w, a, group * 32 * C, 2 * first + half, r32);
 }
 
 // 64 consecutive rows a tile, staged in LDS for up to 8 waves of 64 queries each.  The tiles come by LDS-DMA into a ring of four, three tiles
@@ -520,7 +549,7 @@ __device__ __forceinline__ void mx4_wait_vm_upto(int n)
 	}
 }
 
-template <int KS, bool EXACT>
+template <int KS>
 __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtiles, int splits)
 {
 	extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -529,12 +558,12 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	// blocks with equal blockIdx % 8 share an XCD and its L2: they take the same tiles for their different queries
 	const int j8 = blockIdx.x >> 3, qtile = j8 % qtiles;
 	const int split = (blockIdx.x & 7) + 8 * (j8 / qtiles);
-	const int row_bytes = EXACT ? 32 * KS + (2 * KS + 15) / 16 * 16 : a.row_bytes, ksteps = EXACT ? KS : a.ksteps;
+	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	const int slots = row_bytes / 16, islots = slots | 1;
 	const int tile_bytes = islots * 64 * 16;
 	const int q0 = (qtile * nwaves + wave) * 64;
-	Mx4Queries<KS> w;
-	mx4_load_queries<KS, EXACT>(w, a, q0, 2 * split + half, half, r32, ksteps, row_bytes);
+	Mx4Queries<KS, 2> w;
+	mx4_load_queries(w, a, q0, 2 * split + half, half, r32);
 	const int ntiles = split < a.tiles ? (a.tiles - split + splits - 1) / splits : 0;
 
 	using lds_ptr_t = __attribute__((address_space(3))) void *;
@@ -559,7 +588,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 			const int r = slot / islots, pos = slot - r * islots;
 			const void *src = base + (r * slots + (pos < slots ? pos : 0)) * 16;
 			// a row that is left out has scales 255; past the last row nothing is read
-			const bool off = !((keep >> r) & 1) && (pos >= 2 * ksteps || row0 + r >= a.n);
+			const bool off = !((keep >> r) & 1) && (pos >= 2 * KS || row0 + r >= a.n);
 			src = off ? static_cast<const void *>(g_mx4_nan) : src;
 			__builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
 		}
@@ -573,7 +602,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	asm volatile("" ::: "memory");
 	constexpr bool AHEAD = KS <= 8;  // room in the registers for the fragments of the next 32 rows
 	Mx4Frag<KS> f0, f1;
-	if (AHEAD && ntiles > 0) mx4_load_frag<KS, EXACT>(f0, image(0, 0), half, ksteps);
+	if (AHEAD && ntiles > 0) mx4_load_frag<KS>(f0, image(0, 0), half);
 	for (int t = 0; t < ntiles; t++) {
 		// this wave's share of tile t + 1 is there (loads complete in order; the share of tile t + 2 may be under way) ...
 		mx4_wait_vm_upto(t + 2 < ntiles ? mine : 0);
@@ -582,21 +611,21 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		if (t + 3 < ntiles) fetch(t + 3);
 		const int64_t row0 = mx4_tile_row(a, split + t * splits);
 		mx4_v16f acc[2];
-		if (!AHEAD) mx4_load_frag<KS, EXACT>(f0, image(t, 0), half, ksteps);
+		if (!AHEAD) mx4_load_frag<KS>(f0, image(t, 0), half);
 		if (AHEAD) {
-			mx4_load_frag<KS, EXACT>(f1, image(t, 1), half, ksteps);
+			mx4_load_frag<KS>(f1, image(t, 1), half);
 			__builtin_amdgcn_sched_barrier(0);
 		}
 		mx4_shift_scales(f0, half);
-		mx4_tile<KS, EXACT, 2>(f0, w.b, ksteps, acc);
+		mx4_tile<KS, 2>(f0, w.b, acc);
 		mx4_test(w, a, acc, row0, half);
-		if (!AHEAD) mx4_load_frag<KS, EXACT>(f1, image(t, 1), half, ksteps);
+		if (!AHEAD) mx4_load_frag<KS>(f1, image(t, 1), half);
 		if (AHEAD && t + 1 < ntiles) {
-			mx4_load_frag<KS, EXACT>(f0, image(t + 1, 0), half, ksteps);
+			mx4_load_frag<KS>(f0, image(t + 1, 0), half);
 			__builtin_amdgcn_sched_barrier(0);
 		}
 		mx4_shift_scales(f1, half);
-		mx4_tile<KS, EXACT, 2>(f1, w.b, ksteps, acc);
+		mx4_tile<KS, 2>(f1, w.b, acc);
 		mx4_test(w, a, acc, row0 + 32, half);
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the tile are done before it passes the next barrier
 	}
@@ -605,7 +634,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 
 // The queries that lost keys, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
 // to the best k when the next 128 might not fit.
-template <int KS, bool EXACT>
+template <int KS>
 __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, const int32_t *over, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
@@ -615,7 +644,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 	for (int q = blockIdx.x; q < a.nq; q += gridDim.x) {
 		if (!over[q]) continue;
 		Mx4Frag<KS> b[1];
-		mx4_load_frag<KS, EXACT>(b[0], a.q + (int64_t)q * a.row_bytes, half, a.ksteps);
+		mx4_load_frag<KS>(b[0], a.q + (int64_t)q * mx4_row_bytes(64 * KS), half);
 		mx4_shift_scales(b[0], half);
 		mx4_key kth = 1;  // keys below it are not wanted
 		if (tid == 0) count = 0;
@@ -625,10 +654,10 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 			if (row0 < a.n) {
 				const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
 				Mx4Frag<KS> f;
-				mx4_load_frag<KS, EXACT>(f, a.rows + r * a.row_bytes, half, a.ksteps);
+				mx4_load_frag<KS>(f, a.rows + r * mx4_row_bytes(64 * KS), half);
 				mx4_shift_scales(f, half);
 				mx4_v16f acc[1];
-				mx4_tile<KS, EXACT, 1>(f, b, a.ksteps, acc);
+				mx4_tile<KS, 1>(f, b, acc);
 				if (r32 == 0) {  // every column holds the same query
 #pragma unroll
 					for (int i = 0; i < 16; i++) {
@@ -680,7 +709,7 @@ struct Mx4Plan {
 
 inline size_t mx4_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-inline Mx4Plan mx4_plan(int nq, int n, int k)
+inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 {
 	Mx4Plan p{};
 	p.chunks = nq <= kMx4ChunkQ;
@@ -711,10 +740,12 @@ inline Mx4Plan mx4_plan(int nq, int n, int k)
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
 	p.slab = nq < kMx4SlabQ ? nq : kMx4SlabQ;
 	p.qgroups = (p.slab + 63) / 64;
-	if (p.qgroups > kMx4StreamGroups) {
+	if (p.qgroups > kMx4StreamGroups) {  // (groups of 64)
 		p.qtiles = (p.qgroups + 7) / 8;
 		p.splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles);  // 8 x qtiles workgroups at a time: one a compute unit
 	} else {
+		const int wide = 32 * mx4_stream_frags(mx4_blocks(dim) / 2);
+		p.qgroups = (p.slab + wide - 1) / wide;
 		const int64_t most_waves = kMx4StreamWaves / p.qgroups;
 		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 1) : most_waves);
 	}
@@ -725,10 +756,10 @@ inline Mx4Plan mx4_plan(int nq, int n, int k)
 	return p;
 }
 
-size_t mx4_scan_workspace(int nq, int n, int k) { return mx4_plan(nq, n, k).ws; }
+size_t mx4_scan_workspace(int nq, int n, int dim, int k) { return mx4_plan(nq, n, dim, k).ws; }
 
 // once per kernel and device: how much LDS a launch may ask for
-template <int KS, bool EXACT, int WHICH>
+template <int KS, int WHICH>
 struct Mx4Mark {
 	static inline std::atomic<bool> set[16] = {};
 };
@@ -743,25 +774,26 @@ inline hipError_t mx4_allow_lds(const void *fn, int bytes, std::atomic<bool> (&s
 	return e;
 }
 
-template <int KS, bool EXACT>
-hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, int k, const uint32_t *allow,
+template <int KS>
+hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int k, const uint32_t *allow,
                            const Mx4Out &o, void *ws, hipStream_t s)
 {
 	mx4_key *keys = static_cast<mx4_key *>(ws);
 	const int64_t stride = (int64_t)p.parts * k;
 	const size_t lds = (size_t)nq * p.chunk * 4;
-	const hipError_t e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS, EXACT>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, EXACT, 0>::set);
+	const hipError_t e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, 0>::set);
 	if (e != hipSuccess) return e;
 	if (p.parts > 0)
-		hipLaunchKernelGGL((mx4_chunk_kernel<KS, EXACT>), dim3(p.parts), dim3(256), lds, s, q, nq, rows, n, ksteps, row_bytes, k, p.chunk, allow, keys, stride);
+		hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(p.parts), dim3(kMx4ChunkThreads), lds, s, q, nq, rows, n, k, p.chunk, allow, keys, stride);
 	hipLaunchKernelGGL(mx4_pick_chunks_kernel, dim3(nq), dim3(1024), 0, s, keys, (int)stride, k, o);
 	return hipGetLastError();
 }
 
-template <int KS, bool EXACT>
-hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, int k, const uint32_t *allow,
+template <int KS>
+hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int k, const uint32_t *allow,
                            const Mx4Out &last, void *ws, hipStream_t s)
 {
+	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	uint8_t *w = static_cast<uint8_t *>(ws);
 	auto take = [&](size_t bytes) -> void * {
 		void *at = w;
@@ -780,8 +812,6 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	a.allow = allow;
 	a.nq = nq;
 	a.n = n;
-	a.ksteps = ksteps;
-	a.row_bytes = row_bytes;
 	a.bound = bound;
 	a.parts = p.parts;
 	if (p.levels) {
@@ -794,9 +824,9 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const size_t lds = (size_t)kMx4Ring * mx4_image_slots(row_bytes) * 1024;
 	hipError_t e = hipSuccess;
 	if (p.levels && stage)
-		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS, EXACT>), kMx4Ring * mx4_image_slots(mx4_row_bytes(64 * KS)) * 1024,
-		                  Mx4Mark<KS, EXACT, 1>::set);
-	if (e == hipSuccess) e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, ksteps, row_bytes, scores, m, s);
+		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS>), kMx4Ring * mx4_image_slots(row_bytes) * 1024,
+		                  Mx4Mark<KS, 1>::set);
+	if (e == hipSuccess) e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, KS, row_bytes, scores, m, s);
 	if (e != hipSuccess) return e;
 	hipLaunchKernelGGL(mx4_pick_first_kernel, dim3(nq), dim3(256), 0, s, scores, m, p.step0, n, k, allow, p.levels ? mid : last, (int64_t)kMx4ScanMaxK, over);
 	const int64_t tiles = ((int64_t)n + 63) / 64;
@@ -807,20 +837,20 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 		a.step /= p.ratio;
 		a.tiles = (int)((tiles + a.step - 1) / a.step - before);
 		if (stage)
-			hipLaunchKernelGGL((mx4_stage_kernel<KS, EXACT>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
+			hipLaunchKernelGGL((mx4_stage_kernel<KS>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
 		else
-			hipLaunchKernelGGL((mx4_stream_kernel<KS, EXACT>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
+			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
 		hipLaunchKernelGGL(mx4_pick_kernel, dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, k, l < p.levels ? mid : last, over);
 	}
 	if (p.levels)
-		hipLaunchKernelGGL((mx4_rescue_kernel<KS, EXACT>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
+		hipLaunchKernelGGL((mx4_rescue_kernel<KS>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
 	return hipGetLastError();
 }
 
 hipError_t mx4_launch_scan(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, int k, const uint32_t *allow, int32_t *out_ids,
                            float *out_val, int32_t *out_count, void *ws, hipStream_t s)
 {
-	const Mx4Plan p = mx4_plan(nq, n, k);
+	const Mx4Plan p = mx4_plan(nq, n, dim, k);
 	const int rb = mx4_row_bytes(dim), ks = mx4_blocks(dim) / 2;
 	const int slab = p.chunks ? nq : p.slab;
 	for (int64_t q0 = 0; q0 < nq; q0 += slab) {
@@ -830,11 +860,10 @@ hipError_t mx4_launch_scan(const uint8_t *q, int nq, const uint8_t *rows, int n,
 		o.val = out_val + q0 * k;
 		o.count = out_count + q0;
 		hipError_t e = hipErrorInvalidValue;
-		auto go = [&](auto steps, auto exact) {
+		auto go = [&](auto steps) {
 			constexpr int KS = decltype(steps)::value;
-			constexpr bool EXACT = decltype(exact)::value;
-			e = p.chunks ? mx4_scan_chunks<KS, EXACT>(p, q + q0 * rb, m, rows, n, ks, rb, k, allow, o, ws, s)
-			             : mx4_scan_levels<KS, EXACT>(p, q + q0 * rb, m, rows, n, ks, rb, k, allow, o, ws, s);
+			e = p.chunks ? mx4_scan_chunks<KS>(p, q + q0 * rb, m, rows, n, k, allow, o, ws, s)
+			             : mx4_scan_levels<KS>(p, q + q0 * rb, m, rows, n, k, allow, o, ws, s);
 		};
 		mx4_for_steps(ks, go);
 		if (e != hipSuccess) return e;

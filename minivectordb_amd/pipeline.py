@@ -213,7 +213,10 @@ class ResidentSearcher:
 class ResidentMx4:
     """The microscaled 4-bit operators over device tensors (mvdb_mx4_*_dev; the format is in include/mvdb_hip.h): rows -> packed
     rows, packed rows -> values, every dot product, the k largest dot products.  Everything runs on the caller's current
-    stream of `device`; nothing is kept between calls and nothing synchronises, so calls may be captured into a graph."""
+    stream of `device`; nothing is kept between calls and nothing synchronises, so calls may be captured into a graph.
+
+    A call on a few rows takes the GPU less time than the interpreter, so the methods check their arguments with as few
+    steps as they can and pass plain numbers to the library."""
 
     _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -225,89 +228,107 @@ class ResidentMx4:
             raise MvdbError(f"ResidentMx4: a GPU device is needed, got {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
+        self._raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the objects around it
+        self._cfg = None
+
+    def _engine(self):
+        """The bridge's handle; dim and row_bytes follow it when the bridge is initialised again."""
+        b = self.b
+        if b._cfg is not self._cfg or not b._h:
+            self._dim, self._row_bytes, self._cfg = b._dim(), b.mx4RowBytes(), b._cfg
+        return b._h
 
     @property
     def dim(self) -> int:
-        return self.b._dim()
+        self._engine()
+        return self._dim
 
     @property
     def row_bytes(self) -> int:
-        return self.b.mx4RowBytes()
-
-    def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        self._engine()
+        return self._row_bytes
 
     def _on_device(self, t, what: str):
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._index:
             raise MvdbError(f"{what}: a tensor on {self.device} is needed, got {getattr(t, 'device', type(t).__name__)}")
 
-    def _packed(self, t, what: str):
+    def _packed(self, t, what: str) -> int:
+        """The number of packed rows in t."""
         self._on_device(t, what)
-        if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != self.row_bytes or not t.is_contiguous():
-            raise MvdbError(f"{what}: packed rows are contiguous uint8 [rows, {self.row_bytes}], got {t.dtype} {tuple(t.shape)}")
-        if t.shape[0] > 2**31 - 1:
-            raise MvdbError(f"{what}: {t.shape[0]} rows, at most 2^31 - 1")
-        return t
+        shape = t.shape
+        if t.dtype is not torch.uint8 or len(shape) != 2 or shape[1] != self._row_bytes or not t.is_contiguous():
+            raise MvdbError(f"{what}: packed rows are contiguous uint8 [rows, {self._row_bytes}], got {t.dtype} {tuple(shape)}")
+        if shape[0] > 2147483647:
+            raise MvdbError(f"{what}: {shape[0]} rows, at most 2^31 - 1")
+        return shape[0]
 
     def quantize(self, x: torch.Tensor) -> torch.Tensor:
         """[rows, dim] f32, bf16 or f16 (rows may lie apart, components may not) -> packed rows, uint8 [rows, row_bytes]."""
+        h = self._engine()
         self._on_device(x, "mx4 quantize")
-        if x.dtype not in self._DTYPES:
+        dtype, shape, dim = self._DTYPES.get(x.dtype), x.shape, self._dim
+        if dtype is None:
             raise MvdbError(f"mx4 quantize: float32, bfloat16 or float16 rows are needed, got {x.dtype}")
-        if x.dim() != 2 or x.shape[1] != self.dim:
-            raise MvdbError(f"mx4 quantize: expected rows of dim={self.dim}, got shape {tuple(x.shape)}")
-        rows = x.shape[0]
-        ld = x.stride(0) if rows > 1 else self.dim
-        if x.stride(1) != 1 or ld < self.dim:
+        if len(shape) != 2 or shape[1] != dim:
+            raise MvdbError(f"mx4 quantize: expected rows of dim={dim}, got shape {tuple(shape)}")
+        rows = shape[0]
+        ld, inner = x.stride()
+        if rows <= 1:
+            ld = dim
+        if inner != 1 or ld < dim:
             raise MvdbError(f"mx4 quantize: components have to follow each other and rows not overlap, got strides {x.stride()}")
-        out = torch.empty((rows, self.row_bytes), dtype=torch.uint8, device=self.device)
-        self.b._check(self.L.mvdb_mx4_quantize_dev(self.b.handle, C.c_void_p(x.data_ptr()), self._DTYPES[x.dtype], rows, ld,
-                                                   C.c_void_p(out.data_ptr()), self._stream()))
+        out = torch.empty((rows, self._row_bytes), dtype=torch.uint8, device=self.device)
+        if not self.L.mvdb_mx4_quantize_dev(h, x.data_ptr(), dtype, rows, ld, out.data_ptr(), self._raw_stream(self._index)):
+            self.b._check(0)
         return out
 
     def expand(self, packed: torch.Tensor) -> torch.Tensor:
         """Packed rows -> the values they stand for, f32 [rows, dim]."""
-        self._packed(packed, "mx4 expand")
-        out = torch.empty((packed.shape[0], self.dim), dtype=torch.float32, device=self.device)
-        self.b._check(self.L.mvdb_mx4_expand_dev(self.b.handle, C.c_void_p(packed.data_ptr()), packed.shape[0], C.c_void_p(out.data_ptr()),
-                                                 self._stream()))
+        h = self._engine()
+        rows = self._packed(packed, "mx4 expand")
+        out = torch.empty((rows, self._dim), dtype=torch.float32, device=self.device)
+        if not self.L.mvdb_mx4_expand_dev(h, packed.data_ptr(), rows, out.data_ptr(), self._raw_stream(self._index)):
+            self.b._check(0)
         return out
 
     def product(self, q: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """Every dot product of packed queries and packed rows, f32 [nq, n]; `out` may be a slice with wider rows."""
-        self._packed(q, "mx4 product (queries)")
-        self._packed(rows, "mx4 product (rows)")
-        nq, n = q.shape[0], rows.shape[0]
+        h = self._engine()
+        nq, n = self._packed(q, "mx4 product (queries)"), self._packed(rows, "mx4 product (rows)")
         if out is None:
             out = torch.empty((nq, n), dtype=torch.float32, device=self.device)
-        self._on_device(out, "mx4 product (out)")
-        ldo = out.stride(0) if nq > 1 and out.dim() == 2 else n
-        if out.dtype != torch.float32 or tuple(out.shape) != (nq, n) or (n > 1 and out.stride(1) != 1) or ldo < n:
-            raise MvdbError(f"mx4 product: out has to be float32 [{nq}, {n}] with rows in one piece that do not overlap, got {out.dtype} "
-                            f"{tuple(out.shape)} strides {out.stride()}")
-        self.b._check(self.L.mvdb_mx4_product_dev(self.b.handle, C.c_void_p(q.data_ptr()), nq, C.c_void_p(rows.data_ptr()), n,
-                                                  C.c_void_p(out.data_ptr()), ldo, self._stream()))
+            ldo = n
+        else:
+            self._on_device(out, "mx4 product (out)")
+            ldo = out.stride(0) if nq > 1 and out.dim() == 2 else n
+            if out.dtype != torch.float32 or tuple(out.shape) != (nq, n) or (n > 1 and out.stride(1) != 1) or ldo < n:
+                raise MvdbError(f"mx4 product: out has to be float32 [{nq}, {n}] with rows in one piece that do not overlap, got "
+                                f"{out.dtype} {tuple(out.shape)} strides {out.stride()}")
+        if not self.L.mvdb_mx4_product_dev(h, q.data_ptr(), nq, rows.data_ptr(), n, out.data_ptr(), ldo, self._raw_stream(self._index)):
+            self.b._check(0)
         return out
 
     def scan_many(self, q: torch.Tensor, rows: torch.Tensor, k: int, allow: torch.Tensor | None = None):
         """The k (1..128) largest dot products of each packed query -> (ids i32 [nq, k], values f32 [nq, k], counts i32 [nq]) by (value
         desc, id asc); ids -1 and values 0 behind the count.  allow: bitmap over the rows (int32 words) or None."""
-        self._packed(q, "mx4 scan (queries)")
-        self._packed(rows, "mx4 scan (rows)")
-        nq, n, k = q.shape[0], rows.shape[0], int(k)
+        h = self._engine()
+        nq, n, k = self._packed(q, "mx4 scan (queries)"), self._packed(rows, "mx4 scan (rows)"), int(k)
+        bits = None
         if allow is not None:
             self._on_device(allow, "mx4 scan (allow)")
             if allow.dtype not in (torch.int32, torch.uint32) or allow.dim() != 1 or not allow.is_contiguous() or allow.shape[0] < (n + 31) // 32:
                 raise MvdbError(f"mx4 scan: allow is a bitmap of at least {(n + 31) // 32} int32 words, got {allow.dtype} {tuple(allow.shape)}")
+            bits = allow.data_ptr()
         if not 1 <= k <= 128:
             raise MvdbError(f"mx4 scan: k must be 1..128, got {k}")
-        ids = torch.empty((nq, k), dtype=torch.int32, device=self.device)
-        val = torch.empty((nq, k), dtype=torch.float32, device=self.device)
-        cnt = torch.empty((nq,), dtype=torch.int32, device=self.device)
-        need = self.L.mvdb_mx4_scan_workspace(self.b.handle, nq, n, k)
-        ws = torch.empty((need,), dtype=torch.uint8, device=self.device)
-        vp = C.c_void_p
-        self.b._check(self.L.mvdb_mx4_scan_many_dev(self.b.handle, vp(q.data_ptr()), nq, vp(rows.data_ptr()), n, k,
-                                                    vp(allow.data_ptr()) if allow is not None else None, vp(ids.data_ptr()),
-                                                    vp(val.data_ptr()), vp(cnt.data_ptr()), vp(ws.data_ptr()), need, self._stream()))
+        dev = self.device
+        ids = torch.empty((nq, k), dtype=torch.int32, device=dev)
+        val = torch.empty((nq, k), dtype=torch.float32, device=dev)
+        cnt = torch.empty((nq,), dtype=torch.int32, device=dev)
+        need = self.L.mvdb_mx4_scan_workspace(h, nq, n, k)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        if not self.L.mvdb_mx4_scan_many_dev(h, q.data_ptr(), nq, rows.data_ptr(), n, k, bits, ids.data_ptr(), val.data_ptr(), cnt.data_ptr(),
+                                             ws.data_ptr(), need, self._raw_stream(self._index)):
+            self.b._check(0)
         return ids, val, cnt
