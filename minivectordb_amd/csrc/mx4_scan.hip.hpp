@@ -23,6 +23,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "mx4.hpp"
@@ -420,37 +421,44 @@ __device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS, C> &w, con
 		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = w.count[c];
 }
 
-// Products of 32 rows (row0 ..) with the wave's queries: test, and append what passes.  The test is one maximum over the lane's 16 rows; who
-// passed is looked for four rows at a time.
+// Test of a lane's 16 products with each of its queries: the largest of every four, and whether any may be a candidate.
 template <int KS, int C>
-__device__ __forceinline__ void mx4_test(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], int64_t row0, int half)
+__device__ __forceinline__ bool mx4_test(const Mx4Queries<KS, C> &w, const mx4_v16f (&acc)[C], float (&m)[C][4])
 {
+	bool any = false;
 #pragma unroll
 	for (int c = 0; c < C; c++) {
-		float m[4];
 #pragma unroll
-		for (int g = 0; g < 4; g++) m[g] = __builtin_fmaxf(__builtin_fmaxf(acc[c][4 * g], acc[c][4 * g + 1]), __builtin_fmaxf(acc[c][4 * g + 2], acc[c][4 * g + 3]));
-		const float top = __builtin_fmaxf(__builtin_fmaxf(m[0], m[1]), __builtin_fmaxf(m[2], m[3]));
-		if (__builtin_expect(__ballot(top >= w.bound[c]) != 0, 0)) {
-			unsigned id0 = (unsigned)row0 + 4 * half;
-			asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
+		for (int g = 0; g < 4; g++)
+			m[c][g] = __builtin_fmaxf(__builtin_fmaxf(acc[c][4 * g], acc[c][4 * g + 1]), __builtin_fmaxf(acc[c][4 * g + 2], acc[c][4 * g + 3]));
+		any |= __builtin_fmaxf(__builtin_fmaxf(m[c][0], m[c][1]), __builtin_fmaxf(m[c][2], m[c][3])) >= w.bound[c];
+	}
+	return any;
+}
+
+// Append what passed; rows row0 .. + 31.
+template <int KS, int C>
+__device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], const float (&m)[C][4], int64_t row0, int half)
+{
+	unsigned id0 = (unsigned)row0 + 4 * half;
+	asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
 #pragma unroll
-			for (int g = 0; g < 4; g++)
-				if (__ballot(m[g] >= w.bound[c])) {
+	for (int c = 0; c < C; c++)
 #pragma unroll
-					for (int j = 0; j < 4; j++) {
-						const float v = acc[c][4 * g + j];
-						if (v >= w.bound[c]) {
-							const mx4_key key = mx4_make_key(v, id0 + 8 * g + j);
-							if (key > w.bkey[c]) {
-								if (w.count[c] < kMx4List) a.lists[(size_t)w.list[c] + w.count[c]] = key;
-								w.count[c]++;
-							}
+		for (int g = 0; g < 4; g++)
+			if (__ballot(m[c][g] >= w.bound[c])) {
+#pragma unroll
+				for (int j = 0; j < 4; j++) {
+					const float v = acc[c][4 * g + j];
+					if (v >= w.bound[c]) {
+						const mx4_key key = mx4_make_key(v, id0 + 8 * g + j);
+						if (key > w.bkey[c]) {
+							if (w.count[c] < kMx4List) a.lists[(size_t)w.list[c] + w.count[c]] = key;
+							w.count[c]++;
 						}
 					}
 				}
-		}
-	}
+			}
 }
 
 // fragments of 32 queries a wave of the stream kernel holds
@@ -488,7 +496,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 		mx4_shift_scales(f, half);
 		mx4_v16f acc[C];
 		mx4_tile<KS, C>(f, w.b, acc);
-		mx4_test(w, a, acc, row0, half);
+		float m[C][4];
+		if (__builtin_expect(__ballot(mx4_test(w, acc, m)) != 0, 0)) mx4_append(w, a, acc, m, row0, half);
 	};
 	if constexpr (KS <= 12) {
 		Mx4Frag<KS> f0, f1;
@@ -530,22 +539,26 @@ static __device__ __align__(16) int g_mx4_nan[4] = {-1, -1, -1, -1};  // scales 
 
 __host__ __device__ constexpr int mx4_image_slots(int row_bytes) { return (row_bytes / 16) | 1; }
 
+// Tiles between two barriers, as many as the ring has room for: a wave that appends keeps the others waiting at the barrier, the less the further
+// these are apart (4096 queries, 900 000 x 512, 168 candidates a query: 1 tile 960 us, 2 tiles 880 us).
+__host__ __device__ constexpr int mx4_stage_group(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 2 : 1; }
+
 template <int N>
 __device__ __forceinline__ void mx4_wait_vm()
 {
 	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// until at most n vector-memory operations of this wave are outstanding (n is wave-uniform); more than 6 counts as 0
+// until at most n vector-memory operations of this wave are outstanding (n is wave-uniform); more than MOST counts as 0
+template <int MOST = 12>
 __device__ __forceinline__ void mx4_wait_vm_upto(int n)
 {
-	switch (n) {
-	case 1: mx4_wait_vm<1>(); break;
-	case 2: mx4_wait_vm<2>(); break;
-	case 3: mx4_wait_vm<3>(); break;
-	case 4: mx4_wait_vm<4>(); break;
-	case 5: mx4_wait_vm<5>(); break;
-	case 6: mx4_wait_vm<6>(); break;
-	default: mx4_wait_vm<0>(); break;
+	if constexpr (MOST == 0) {
+		mx4_wait_vm<0>();
+	} else {
+		if (n == MOST)
+			mx4_wait_vm<MOST>();
+		else
+			mx4_wait_vm_upto<MOST - 1>(n);
 	}
 }
 
@@ -572,7 +585,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	auto fetch = [&](int t) {
 		const int64_t row0 = mx4_tile_row(a, split + t * splits);
 		const uint8_t *base = a.rows + row0 * row_bytes;
-		unsigned char *dst = lds + (t & (kMx4Ring - 1)) * tile_bytes;
+		unsigned char *dst = lds + (t & (kMx4Ring * mx4_stage_group(KS) - 1)) * tile_bytes;
 		if (islots == slots && !a.allow && row0 + 64 <= a.n) {  // the image is the tile as it lies in memory
 			for (int i = wave; i < islots; i += nwaves)
 				__builtin_amdgcn_global_load_lds((glb_ptr_t)(base + i * 1024 + (unsigned)lane * 16), (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
@@ -594,40 +607,88 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		}
 	};
 	const int mine = (islots - wave + nwaves - 1) / nwaves;  // instructions of a fetch by this wave
-	auto image = [&](int t, int h) -> const unsigned char * { return lds + (t & (kMx4Ring - 1)) * tile_bytes + (h * 32 + r32) * islots * 16; };
+	constexpr int G = mx4_stage_group(KS);
+	auto image = [&](int t, int h) -> const unsigned char * { return lds + (t & (kMx4Ring * G - 1)) * tile_bytes + (h * 32 + r32) * islots * 16; };
 	mx4_wait_vm<0>();
-	for (int t = 0; t < 3 && t < ntiles; t++) fetch(t);
-	mx4_wait_vm_upto(ntiles > 2 && 2 * mine <= 6 ? 2 * mine : 0);  // this wave's share of tile 0
+	for (int t = 0; t < 3 * G && t < ntiles; t++) fetch(t);
+	mx4_wait_vm_upto(0);  // (once)
 	__builtin_amdgcn_s_barrier();
 	asm volatile("" ::: "memory");
 	constexpr bool AHEAD = KS <= 8;  // room in the registers for the fragments of the next 32 rows
 	Mx4Frag<KS> f0, f1;
 	if (AHEAD && ntiles > 0) mx4_load_frag<KS>(f0, image(0, 0), half);
-	for (int t = 0; t < ntiles; t++) {
-		// this wave's share of tile t + 1 is there (loads complete in order; the share of tile t + 2 may be under way) ...
-		mx4_wait_vm_upto(t + 2 < ntiles ? mine : 0);
-		__builtin_amdgcn_s_barrier();  // ... and everybody's, and tile t - 1 is done with
+	constexpr bool PIPED = KS <= 12;
+	// Two sets of accumulators (where there is room): the products of one 32 rows are tested while those of the next are computed.
+	mx4_v16f accA[2], accB[2];
+#pragma unroll
+	for (int c = 0; c < 2; c++)
+#pragma unroll
+		for (int i = 0; i < 16; i++) accB[c][i] = __uint_as_float(0x7fc00000u);
+	int64_t rowB = 0;
+	auto step = [&](Mx4Frag<KS> &f, mx4_v16f (&now)[2], mx4_v16f (&then)[2], int64_t row) {
+		mx4_shift_scales(f, half);
+		if constexpr (!PIPED) {
+			mx4_tile<KS, 2>(f, w.b, now);
+			float m[2][4];
+			if (__builtin_expect(__ballot(mx4_test(w, now, m)) != 0, 0)) mx4_append(w, a, now, m, row, half);
+			return;
+		}
+		const mx4_v16f zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+		float m[2][4];
+#pragma unroll
+		for (int s = 0; s < KS; s++) {
+#pragma unroll
+			for (int c = 0; c < 2; c++) {
+				const mx4_v16f &in = s == 0 ? zero : now[c];
+				now[c] = (s & 1) ? mx4_mfma<2, 2>(f.d[s], f.sc[s / 2], w.b[c].d[s], w.b[c].sc[s / 2], in)
+				                 : mx4_mfma<0, 0>(f.d[s], f.sc[s / 2], w.b[c].d[s], w.b[c].sc[s / 2], in);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+			for (int p = s * 8 / KS; p < (s + 1) * 8 / KS; p++) {  // a share of the test behind every two matrix instructions
+				const int c = p >> 2, g = p & 3;
+				m[c][g] = __builtin_fmaxf(__builtin_fmaxf(then[c][4 * g], then[c][4 * g + 1]), __builtin_fmaxf(then[c][4 * g + 2], then[c][4 * g + 3]));
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		}
+#pragma unroll
+		for (int c = 0; c < 2; c++) asm volatile("" : "+v"(now[c]));  // see mx4_tile
+		bool any = false;
+#pragma unroll
+		for (int c = 0; c < 2; c++) any |= __builtin_fmaxf(__builtin_fmaxf(m[c][0], m[c][1]), __builtin_fmaxf(m[c][2], m[c][3])) >= w.bound[c];
+		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append(w, a, then, m, row, half);
+	};
+	for (int t = 0; t < ntiles; t += G) {
+		// this wave's share of the next G tiles is there (loads complete in order; the G after them may be under way) ...
+		mx4_wait_vm_upto(t + 3 * G <= ntiles ? G * mine : 0);
+		__builtin_amdgcn_s_barrier();  // ... and everybody's, and the G before these are done with
 		asm volatile("" ::: "memory");
-		if (t + 3 < ntiles) fetch(t + 3);
-		const int64_t row0 = mx4_tile_row(a, split + t * splits);
-		mx4_v16f acc[2];
-		if (!AHEAD) mx4_load_frag<KS>(f0, image(t, 0), half);
-		if (AHEAD) {
-			mx4_load_frag<KS>(f1, image(t, 1), half);
-			__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int g = 0; g < G; g++)
+			if (t + 3 * G + g < ntiles) fetch(t + 3 * G + g);
+#pragma unroll
+		for (int g = 0; g < G; g++) {
+			if (g > 0 && t + g >= ntiles) break;
+			const int64_t row0 = mx4_tile_row(a, split + (t + g) * splits);
+			if (!AHEAD) mx4_load_frag<KS>(f0, image(t + g, 0), half);
+			if (AHEAD) {
+				mx4_load_frag<KS>(f1, image(t + g, 1), half);
+				__builtin_amdgcn_sched_barrier(0);
+			}
+			step(f0, accA, accB, PIPED ? rowB : row0);
+			if (!AHEAD) mx4_load_frag<KS>(f1, image(t + g, 1), half);
+			if (AHEAD && t + g + 1 < ntiles) {
+				mx4_load_frag<KS>(f0, image(t + g + 1, 0), half);
+				__builtin_amdgcn_sched_barrier(0);
+			}
+			step(f1, PIPED ? accB : accA, accA, PIPED ? row0 : row0 + 32);
+			rowB = row0 + 32;
 		}
-		mx4_shift_scales(f0, half);
-		mx4_tile<KS, 2>(f0, w.b, acc);
-		mx4_test(w, a, acc, row0, half);
-		if (!AHEAD) mx4_load_frag<KS>(f1, image(t, 1), half);
-		if (AHEAD && t + 1 < ntiles) {
-			mx4_load_frag<KS>(f0, image(t + 1, 0), half);
-			__builtin_amdgcn_sched_barrier(0);
-		}
-		mx4_shift_scales(f1, half);
-		mx4_tile<KS, 2>(f1, w.b, acc);
-		mx4_test(w, a, acc, row0 + 32, half);
-		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the tile are done before it passes the next barrier
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the tiles are done before it passes the next barrier
+	}
+	if (PIPED) {
+		float m[2][4];
+		if (__ballot(mx4_test(w, accB, m))) mx4_append(w, a, accB, m, rowB, half);
 	}
 	mx4_store_counts(w, a, q0, 2 * split + half, r32);
 }
@@ -697,6 +758,10 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 constexpr int kMx4SlabQ = 8192;       // queries that are dealt with at a time
 constexpr int kMx4StreamGroups = 4;   // up to so many groups of 64 queries: mx4_stream_kernel, more: mx4_stage_kernel
 constexpr int kMx4StreamWaves = 2048;
+#ifndef MX4_R
+#define MX4_R 10
+#endif
+constexpr int kMx4MostRatio = MX4_R;
 
 struct Mx4Plan {
 	bool chunks;
@@ -722,8 +787,9 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 		return p;
 	}
 	const int64_t tiles = ((int64_t)n + 63) / 64;
-	// k (ratio - 1) keys are expected of a level: at most a quarter of what a query can gather
-	const int most = kMx4Gather / 4 / k < 4 ? 4 : kMx4Gather / 4 / k > 10 ? 10 : kMx4Gather / 4 / k;
+	// About k (ratio - 1) keys are expected of a level, with a standard deviation of ratio sqrt(k): a query gathers that and 8 deviations
+	int most = kMx4MostRatio;
+	while (most > 4 && k * (most - 1) + 8 * most * (int)std::ceil(std::sqrt((double)k)) > kMx4Gather - k) most--;
 	p.levels = 0;
 	p.ratio = 0;
 	p.step0 = 1;
@@ -821,10 +887,10 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const Mx4Out mid = {nullptr, nullptr, nullptr, best, bound, nbest};
 	const bool stage = p.qtiles > 0;
 	const int nwaves = stage ? (p.qgroups + p.qtiles - 1) / p.qtiles : 0;
-	const size_t lds = (size_t)kMx4Ring * mx4_image_slots(row_bytes) * 1024;
+	const size_t lds = (size_t)kMx4Ring * mx4_stage_group(KS) * mx4_image_slots(row_bytes) * 1024;
 	hipError_t e = hipSuccess;
 	if (p.levels && stage)
-		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS>), kMx4Ring * mx4_image_slots(row_bytes) * 1024,
+		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS>), (int)lds,
 		                  Mx4Mark<KS, 1>::set);
 	if (e == hipSuccess) e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, KS, row_bytes, scores, m, s);
 	if (e != hipSuccess) return e;
