@@ -64,17 +64,13 @@ struct Mx4Product {
 	int nq, n;
 	float *out;
 	int64_t ldo;
-	int groups, cols, run;  // groups of 32 * mx4_product_frags queries; columns; steps of 128 columns a workgroup
+	int groups, run;  // groups of 32 * mx4_product_frags queries; steps of 128 rows a workgroup
 	int block;              // chunks of an XCD that are gone through for one group of queries after the other
-	int64_t step;
 };
 
 // fragments of 32 queries a wave holds: as many as leave room in its registers for the rows
 __host__ __device__ constexpr int mx4_product_frags(int ks) { return ks <= 8 ? 2 : 1; }
 
-// Column c of the result is row c, or (step > 1) row 64 * step * (c / 64) + c % 64: the 64-row tiles that are multiples of step.  Columns past the
-// last row hold products that nobody reads.
-//
 // Bound by the writing of the result (4 bytes for every 2 * dim operations).  A wave holds 64 queries (32 where rows are long) in registers and takes 32 rows at a time, the
 // next ones on their way meanwhile; the four waves of a workgroup take neighbouring rows, so that together they write 512 bytes of each of 64
 // result rows.  Queries are the rows of D, so a store writes 128 bytes of two result rows.  The workgroups of one XCD go through a block of
@@ -89,7 +85,7 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 	const int64_t chunk = ((int64_t)(j8 / (a.groups * a.block)) * a.block + j % a.block) * 8 + (blockIdx.x & 7);
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	int64_t col0 = chunk * a.run * 128 + wave * 32;
-	if (col0 >= a.cols) return;
+	if (col0 >= a.n) return;
 	constexpr int C = mx4_product_frags(KS);
 	const int q0 = group * 32 * C;
 	Mx4Frag<KS> qf[C];
@@ -98,9 +94,9 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 		const int q = q0 + c * 32 + r32;
 		mx4_load_frag<KS>(qf[c], a.q + (int64_t)(q < a.nq ? q : a.nq - 1) * row_bytes, half);
 	}
-	const int64_t end = (chunk + 1) * a.run * 128 < a.cols ? (chunk + 1) * a.run * 128 : a.cols;
+	const int64_t end = (chunk + 1) * a.run * 128 < a.n ? (chunk + 1) * a.run * 128 : a.n;
 	auto load = [&](int64_t col, Mx4Frag<KS> &f) {
-		const int64_t at = (col & ~(int64_t)63) * a.step + (col & 63) + r32;
+		const int64_t at = col + r32;
 		mx4_load_frag<KS>(f, a.rows + (at < a.n ? at : a.n - 1) * row_bytes, half);
 	};
 	auto use = [&](int64_t col, Mx4Frag<KS> &f) {
@@ -118,7 +114,7 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 			}
 #pragma unroll
 		for (int c = 0; c < C; c++) asm volatile("" : "+v"(acc[c]));  // see mx4_tile
-		const bool full = q0 + 32 * C <= a.nq && col + 32 <= a.cols;
+		const bool full = q0 + 32 * C <= a.nq && col + 32 <= a.n;
 		float *o = a.out + (q0 + 4 * half) * a.ldo + col + r32;
 		if (full) {
 #pragma unroll
@@ -131,7 +127,7 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 					else
 						*p = acc[c][i];
 				}
-		} else if (col + r32 < a.cols) {
+		} else if (col + r32 < a.n) {
 #pragma unroll
 			for (int c = 0; c < C; c++)
 #pragma unroll
@@ -178,20 +174,19 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(Mx4Product a)
 
 // Rows of more than 16 steps (dim > 1024): a wave computes 64 queries x 64 rows, a workgroup (2 x 2 waves) 128 x 128, both operands step by step
 __global__ __launch_bounds__(256) void mx4_product_long_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int ksteps, int row_bytes, float *out,
-                                                          int64_t ldo, int qtiles, int cols, int64_t step)
+                                                               int64_t ldo, int qtiles)
 {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 	const int half = lane >> 5, r32 = lane & 31;
 	const int qt = blockIdx.x % qtiles, rt = blockIdx.x / qtiles;
 	const int q0 = qt * 128 + (wave >> 1) * 64, r0 = rt * 128 + (wave & 1) * 64;
-	if (q0 >= nq || r0 >= cols) return;
+	if (q0 >= nq || r0 >= n) return;
 	const uint8_t *qp[2], *rp[2];
 #pragma unroll
 	for (int t = 0; t < 2; t++) {
-		const int qi = q0 + t * 32 + r32, col = r0 + t * 32 + r32;
-		const int64_t ri = col + (int64_t)(col & ~63) * (step - 1);
+		const int qi = q0 + t * 32 + r32, ri = r0 + t * 32 + r32;
 		qp[t] = q + (int64_t)(qi < nq ? qi : nq - 1) * row_bytes;
-		rp[t] = rows + (ri < n ? ri : n - 1) * row_bytes;
+		rp[t] = rows + (int64_t)(ri < n ? ri : n - 1) * row_bytes;
 	}
 	mx4_v16f acc[2][2];
 #pragma unroll
@@ -224,7 +219,7 @@ __global__ __launch_bounds__(256) void mx4_product_long_kernel(const uint8_t *q,
 #pragma unroll
 			for (int i = 0; i < 16; i++) {
 				const int qi = q0 + t * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-				if (qi < nq && col < cols) out[qi * ldo + col] = acc[t][u][i];
+				if (qi < nq && col < n) out[qi * ldo + col] = acc[t][u][i];
 			}
 		}
 }
@@ -234,20 +229,17 @@ constexpr int kMx4ProductGroups = 4096;  // workgroups a launch, about
 constexpr int64_t kMx4BlockBytes = 4 << 20;  // rows of a block: an XCD's L2
 constexpr int64_t kMx4StreamBytes = 256 << 20;  // results that are larger than the caches go past them
 
-// `cols` columns
-inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8_t *rows, int n, int cols, int64_t step, int ksteps, int row_bytes, float *out,
-                                           int64_t ldo, hipStream_t s)
+hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, float *out, int64_t ldo, hipStream_t s)
 {
-	const int64_t rtiles = ((int64_t)cols + 127) / 128;
-	if (ksteps <= 16) {
+	constexpr int row_steps = 16;  // rows that mx4_product_kernel holds in registers
+	const int ksteps = mx4_blocks(dim) / 2, row_bytes = mx4_row_bytes(dim);
+	const int64_t rtiles = ((int64_t)n + 127) / 128;
+	if (ksteps <= row_steps) {
 		Mx4Product a{};
-		a.q = q;
 		a.rows = rows;
 		a.n = n;
 		a.ldo = ldo;
-		a.cols = cols;
-		a.step = step;
-		const bool stream = (int64_t)nq * cols * 4 > kMx4StreamBytes;
+		const bool stream = (int64_t)nq * n * 4 > kMx4StreamBytes;
 		for (int64_t q0 = 0; q0 < nq; q0 += kMx4ProductQ) {
 			a.nq = (int)(nq - q0 < kMx4ProductQ ? nq - q0 : kMx4ProductQ);
 			a.q = q + q0 * row_bytes;
@@ -255,7 +247,7 @@ inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8
 			const int frags = mx4_product_frags(ksteps);
 			a.groups = (a.nq + 32 * frags - 1) / (32 * frags);
 			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries; but all of a small result's at once
-			int64_t run = rtiles * a.groups / kMx4ProductGroups;
+			const int64_t run = rtiles * a.groups / kMx4ProductGroups;
 			a.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
 			const int64_t chunks = (rtiles + a.run - 1) / a.run;
 			const int64_t per_xcd = (chunks + 7) / 8, fit = kMx4BlockBytes / ((int64_t)a.run * 128 * row_bytes);
@@ -265,7 +257,7 @@ inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8
 			const int64_t blocks = (per_xcd + a.block - 1) / a.block * a.block * 8 * a.groups;
 			mx4_for_steps(ksteps, [&](auto steps) {
 				constexpr int KS = decltype(steps)::value;
-					if (stream)
+				if (stream)
 					hipLaunchKernelGGL((mx4_product_kernel<KS, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
 				else
 					hipLaunchKernelGGL((mx4_product_kernel<KS, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -273,24 +265,16 @@ inline hipError_t mx4_launch_product_tiles(const uint8_t *q, int nq, const uint8
 		}
 		return hipGetLastError();
 	}
-	const int64_t qstep = 1 << 16;  // queries a launch (what one grid can hold)
-	for (int64_t q0 = 0; q0 < nq; q0 += qstep) {
-		const int m = (int)(nq - q0 < qstep ? nq - q0 : qstep), qtiles = (m + 127) / 128;
-		const int64_t rstep = ((int64_t)1 << 22) / qtiles;
+	for (int64_t q0 = 0; q0 < nq; q0 += kMx4ProductQ) {
+		const int m = (int)(nq - q0 < kMx4ProductQ ? nq - q0 : kMx4ProductQ), qtiles = (m + 127) / 128;
+		const int64_t rstep = ((int64_t)1 << 22) / qtiles;  // what one grid can hold
 		for (int64_t r0 = 0; r0 < rtiles; r0 += rstep) {
 			const int64_t c = rtiles - r0 < rstep ? rtiles - r0 : rstep;
-			const int64_t col = r0 * 128, row = col * step;
-			if (row >= n) break;
-			hipLaunchKernelGGL(mx4_product_long_kernel, dim3((unsigned)(c * qtiles)), dim3(256), 0, s, q + q0 * row_bytes, m, rows + row * row_bytes,
-			                   (int)(n - row), ksteps, row_bytes, out + q0 * ldo + col, ldo, qtiles, (int)(cols - col), step);
+			hipLaunchKernelGGL(mx4_product_long_kernel, dim3((unsigned)(c * qtiles)), dim3(256), 0, s, q + q0 * row_bytes, m, rows + r0 * 128 * row_bytes,
+			                   (int)(n - r0 * 128), ksteps, row_bytes, out + q0 * ldo + r0 * 128, ldo, qtiles);
 		}
 	}
 	return hipGetLastError();
-}
-
-hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int n, int dim, float *out, int64_t ldo, hipStream_t s)
-{
-	return mx4_launch_product_tiles(q, nq, rows, n, n, 1, mx4_blocks(dim) / 2, mx4_row_bytes(dim), out, ldo, s);
 }
 
 }  // namespace mvdb

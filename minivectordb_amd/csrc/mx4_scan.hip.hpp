@@ -14,7 +14,7 @@
 // ratio^L-th tile, level l the tiles that are multiples of ratio^(L - l) and not of ratio^(L - l + 1).  After a level the k-th best key so
 // far is a bound: k rows are at least that good, so only keys above it matter, and as the rows seen so far are spread evenly over the
 // store about k (ratio - 1) keys of the next level are (whatever order the rows are in, unless they repeat with the tiles' period).
-// Level 0 has no bound: its products go to memory.  From then on a lane whose product passes the bound appends the key to a list of its
+// Level 0 has no bound: it is one chunk.  From then on a lane whose product passes the bound appends the key to a list of its
 // own, which needs no atomics: a lane only ever sees one query a fragment, and the tiles are dealt out in turn, so lists stay short.
 // mx4_pick_kernel gathers a query's lists after every level and keeps the best k.  A list that overflows marks its query, and
 // mx4_rescue_kernel does those over, one workgroup each.
@@ -47,131 +47,214 @@ __device__ __forceinline__ float mx4_key_value(mx4_key key)
 __device__ __forceinline__ int mx4_key_id(mx4_key key) { return (int)~(unsigned)key; }
 
 // ---------------------------------------------------------------------------------------------- selection
-// LDS of mx4_block_kth
-struct Mx4PickLds {
+constexpr int kMx4Best = 256;  // candidates that are put in order by counting, at most
+
+struct __attribute__((aligned(16))) Mx4PickLds {
+	mx4_key best[kMx4Best + 8];
 	int hist[256];
-	mx4_key lo[16], hi[16];  // per wave
-	int pick, above, total;
+	unsigned lo[16], hi[16];  // per wave
+	int pick, above, in_bin, total, count;
 };
 
-// The k-th largest of the keys key_at(0 .. m) (0 = none) of a workgroup of T threads: the key that exactly min(k, keys) are >= to; 1 where
-// there are at most k.  Radix selection, eight bits at a time from the highest bit in which the keys differ: scores lie within a few powers of
-// two, so their leading bits would all fall into one bin.  It ends as soon as a bin is wanted whole.
-template <int T, typename F>
-__device__ mx4_key mx4_block_kth(F key_at, int m, int k, Mx4PickLds &l)
+// Barrier of the T threads that share a selection.  The LDS operations of one wave execute in order, so a wave alone needs none.
+template <int T>
+__device__ __forceinline__ void mx4_sync()
 {
-	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-	mx4_key lo = ~0ull, hi = 0;
-	int have = 0;
-	for (int i = tid; i < m; i += T) {
-		const mx4_key key = key_at(i);
-		if (key) {
-			lo = key < lo ? key : lo;
-			hi = key > hi ? key : hi;
-			have++;
+	if constexpr (T > 64)
+		__syncthreads();
+	else
+		asm volatile("" ::: "memory");
+}
+
+// over the 64 lanes of a wave, by row shifts and broadcasts (no LDS): the largest value, and the inclusive prefix sum
+template <int CTRL>
+__device__ __forceinline__ unsigned mx4_dpp_max(unsigned x)
+{
+	const unsigned y = (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
+	return y > x ? y : x;
+}
+__device__ __forceinline__ unsigned mx4_wave_max(unsigned x)
+{
+	x = mx4_dpp_max<0x111>(x);
+	x = mx4_dpp_max<0x112>(x);
+	x = mx4_dpp_max<0x114>(x);
+	x = mx4_dpp_max<0x118>(x);
+	x = mx4_dpp_max<0x142>(x);
+	x = mx4_dpp_max<0x143>(x);
+	return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ int mx4_wave_scan(int x)
+{
+	x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+	return x;
+}
+
+// The bin, from above, of the need-th key in l.hist (wave 0): l.pick, the keys above it and in it, and all there are
+__device__ __forceinline__ void mx4_find_bin(Mx4PickLds &l, int need, int lane)
+{
+	int c[4], sum = 0;  // lane l has the bins 255 - 4 l down to 252 - 4 l
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		c[j] = l.hist[255 - 4 * lane - j];
+		sum += c[j];
+	}
+	const int upto = mx4_wave_scan(sum);
+	int higher = upto - sum;
+	if (lane == 63) l.total = upto;
+#pragma unroll
+	for (int j = 0; j < 4; j++) {
+		if (higher < need && higher + c[j] >= need) {
+			l.pick = 255 - 4 * lane - j;
+			l.above = higher;
+			l.in_bin = c[j];
 		}
-	}
-	if (tid == 0) l.total = 0;
-#pragma unroll
-	for (int d = 32; d >= 1; d >>= 1) {
-		const mx4_key ol = ((mx4_key)(unsigned)__shfl_xor((int)(lo >> 32), d, 64) << 32) | (unsigned)__shfl_xor((int)(unsigned)lo, d, 64);
-		const mx4_key oh = ((mx4_key)(unsigned)__shfl_xor((int)(hi >> 32), d, 64) << 32) | (unsigned)__shfl_xor((int)(unsigned)hi, d, 64);
-		lo = ol < lo ? ol : lo;
-		hi = oh > hi ? oh : hi;
-		have += __shfl_xor(have, d, 64);
-	}
-	__syncthreads();
-	if (lane == 0) {
-		l.lo[wave] = lo;
-		l.hi[wave] = hi;
-		atomicAdd(&l.total, have);
-	}
-	__syncthreads();
-#pragma unroll
-	for (int w = 0; w < T / 64; w++) {
-		lo = l.lo[w] < lo ? l.lo[w] : lo;
-		hi = l.hi[w] > hi ? l.hi[w] : hi;
-	}
-	if (l.total <= k) return 1;
-	// (more than k keys, so two at least, all different: hi != lo)
-	int top = 64 - __builtin_clzll(hi ^ lo);  // bits [0, top) differ
-	mx4_key fixed = top < 64 ? hi >> top << top : 0;
-	int need = k;
-	while (true) {
-		const int shift = top > 8 ? top - 8 : 0;
-		const unsigned bins = 1u << (top - shift);
-		for (int i = tid; i < 256; i += T) l.hist[i] = 0;
-		__syncthreads();
-		for (int i = tid; i < m; i += T) {
-			const mx4_key key = key_at(i);
-			if (key && (top == 64 || (key >> top) == (fixed >> top))) atomicAdd(&l.hist[(unsigned)(key >> shift) & (bins - 1)], 1);
-		}
-		__syncthreads();
-		if (wave == 0) {  // the bin that holds the need-th from above
-			int c[4], s = 0;
-#pragma unroll
-			for (int j = 3; j >= 0; j--) {
-				s += l.hist[lane * 4 + j];
-				c[j] = s;  // keys in the bins of this lane from j up
-			}
-			int above = s;  // inclusive suffix sum over the lanes
-#pragma unroll
-			for (int d = 1; d < 64; d <<= 1) {
-				const int o = __shfl_down(above, d, 64);
-				above += lane + d < 64 ? o : 0;
-			}
-			above -= s;  // keys in the lanes above
-#pragma unroll
-			for (int j = 0; j < 4; j++) {
-				const int higher = above + (j < 3 ? c[j + 1 < 4 ? j + 1 : 3] : 0);
-				if (higher < need && above + c[j] >= need) {
-					l.pick = lane * 4 + j;
-					l.above = higher;
-				}
-			}
-		}
-		__syncthreads();
-		const int bin = l.pick, in_bin = l.hist[bin];
-		need -= l.above;
-		fixed |= (mx4_key)bin << shift;
-		top = shift;
-		__syncthreads();
-		if (in_bin == need || shift == 0) return fixed;
+		higher += c[j];
 	}
 }
 
-// What a selection does with the best k: the caller's arrays, or (a level that is not the last) back into the buffer, with the k-th as
-// the bound of the next level.  The keys >= the k-th are gathered in LDS and put in order by their rank (they are all different).
+// The best of the keys that T threads (a workgroup, or a wave of one) hold, N a thread (0 = none): l.best[0 .. returned count), in no order, has the best
+// min(k, keys) of them, and at most kMx4Best.  A histogram over 256 equal steps from the smallest value to the largest gives the step of the
+// k-th key, and everything from that step up is the answer: the best of a few thousand products lie far apart, so that is a few keys more than k
+// (and few atomics meet in a bin).  Where it is too many, or the values are not finite, the keys are looked at bit by bit instead, eight at a time
+// from the highest in which the values differ, until few enough share the k-th key's.
+// l.best is written before the last barrier in here; the caller's next one has to come before l is used again.
+template <int T, int N>
+__device__ int mx4_block_best(const mx4_key (&key)[N], int k, Mx4PickLds &l)
+{
+	const int tid = threadIdx.x & (T - 1), lane = tid & 63, wave = tid >> 6;
+	unsigned hi = 0, nlo = 0;  // of the values: the largest, and the largest complement
+#pragma unroll
+	for (int j = 0; j < N; j++) {
+		const unsigned v = (unsigned)(key[j] >> 32);
+		hi = key[j] && v > hi ? v : hi;
+		nlo = key[j] && ~v > nlo ? ~v : nlo;
+	}
+	hi = mx4_wave_max(hi);
+	nlo = mx4_wave_max(nlo);
+	if (lane == 0) {
+		l.hi[wave] = hi;
+		l.lo[wave] = nlo;
+	}
+	for (int i = tid; i < 256; i += T) l.hist[i] = 0;
+	if (tid == 0) l.count = 0;
+	mx4_sync<T>();
+#pragma unroll
+	for (int w = 0; w < T / 64; w++) {
+		hi = l.hi[w] > hi ? l.hi[w] : hi;
+		nlo = l.lo[w] > nlo ? l.lo[w] : nlo;
+	}
+	const float most = mx4_key_value((mx4_key)hi << 32), least = mx4_key_value((mx4_key)~nlo << 32), span = most - least;
+	bool done = false;
+	if (hi != 0 && span > 0.f && span < 3e38f) {
+		const float scale = 255.f / span;  // (subtraction, product and conversion keep the order of the values)
+		int bin[N];
+#pragma unroll
+		for (int j = 0; j < N; j++) {
+			const int x = (int)((mx4_key_value(key[j]) - least) * scale);
+			bin[j] = key[j] ? (x < 255 ? x : 255) : -1;
+			if (bin[j] >= 0) atomicAdd(&l.hist[bin[j]], 1);
+		}
+		mx4_sync<T>();
+		if (wave == 0) mx4_find_bin(l, k, lane);
+		mx4_sync<T>();
+		const int from = l.total < k ? 0 : l.pick;
+		if (l.total < k || l.above + l.in_bin <= kMx4Best) {
+#pragma unroll
+			for (int j = 0; j < N; j++)
+				if (bin[j] >= from) l.best[atomicAdd(&l.count, 1)] = key[j];
+			done = true;
+		} else {
+			mx4_sync<T>();
+			for (int i = tid; i < 256; i += T) l.hist[i] = 0;
+			mx4_sync<T>();
+		}
+	}
+	if (!done) {
+		const unsigned differ = hi ^ ~nlo;
+		int top = hi == 0 || differ == 0 ? 32 : 64 - __builtin_clz(differ);  // bits [0, top) differ
+		mx4_key from = hi == 0 || top == 64 ? 0 : (mx4_key)hi << 32 >> top << top;  // the bits above them
+		int need = k, above = 0;
+		while (true) {
+			const int shift = top > 8 ? top - 8 : 0;
+			const unsigned bins = 1u << (top - shift);
+#pragma unroll
+			for (int j = 0; j < N; j++)
+				if (key[j] && (top == 64 || (key[j] >> top) == (from >> top))) atomicAdd(&l.hist[(unsigned)(key[j] >> shift) & (bins - 1)], 1);
+			mx4_sync<T>();
+			if (wave == 0) mx4_find_bin(l, need, lane);
+			mx4_sync<T>();
+			if (l.total < need) {  // fewer than k keys: all of them
+				from = 1;
+				break;
+			}
+			const int in_bin = l.in_bin;
+			above += l.above;
+			need -= l.above;
+			from |= (mx4_key)l.pick << shift;
+			top = shift;
+			if (above + in_bin <= kMx4Best || shift == 0) break;
+			mx4_sync<T>();
+			for (int i = tid; i < 256; i += T) l.hist[i] = 0;
+			mx4_sync<T>();
+		}
+#pragma unroll
+		for (int j = 0; j < N; j++)
+			if (key[j] && key[j] >= from) l.best[atomicAdd(&l.count, 1)] = key[j];
+	}
+	mx4_sync<T>();
+	return l.count;
+}
+
+// What a selection does with the best k: the caller's arrays, or (a level that is not the last) kept for the next, with the k-th as its bound.
 struct Mx4Out {
 	int32_t *ids, *count;
 	float *val;
-	mx4_key *keys, *bound;  // keys != nullptr: not the last level
+	mx4_key *keys, *bound;  // keys != nullptr: not the last level; [.][kMx4ScanMaxK]
 	int32_t *fill;
 };
 
-template <int T, typename F>
-__device__ void mx4_block_topk(F key_at, int m, int k, int64_t q, int64_t stride, const Mx4Out &o, Mx4PickLds &l, mx4_key *best)
+// how many of the `have` keys in l.best (followed by zeros up to a multiple of 8) are larger
+__device__ __forceinline__ int mx4_rank(const Mx4PickLds &l, int have, mx4_key key)
 {
-	const int tid = threadIdx.x;
-	const mx4_key kth = mx4_block_kth<T>(key_at, m, k, l);
-	if (tid == 0) l.pick = 0;
-	__syncthreads();
-	for (int i = tid; i < m; i += T) {
-		const mx4_key key = key_at(i);
-		if (key >= kth) best[atomicAdd(&l.pick, 1)] = key;  // (kth >= 1)
+	int at = 0;
+	for (int j = 0; j < have; j += 8) {
+		ulonglong2 b[4];
+#pragma unroll
+		for (int i = 0; i < 4; i++) b[i] = *reinterpret_cast<const ulonglong2 *>(&l.best[j + 2 * i]);
+#pragma unroll
+		for (int i = 0; i < 4; i++) at += (b[i].x > key ? 1 : 0) + (b[i].y > key ? 1 : 0);
 	}
-	__syncthreads();
-	const int have = l.pick;  // <= k <= kMx4ScanMaxK
-	for (int i = tid; i < k; i += T) {
+	return at;
+}
+template <int T>
+__device__ __forceinline__ void mx4_pad_best(Mx4PickLds &l, int have)
+{
+	const int tid = threadIdx.x & (T - 1);
+	if (tid < 8) l.best[have + tid] = 0;
+	mx4_sync<T>();
+}
+
+// The best k of the `have` keys in l.best to query q's place, in order: a key's place is the number of larger ones (no two are the same).
+template <int T>
+__device__ void mx4_block_put(int have, int k, int64_t q, const Mx4Out &o, Mx4PickLds &l)
+{
+	const int tid = threadIdx.x & (T - 1), out = have < k ? have : k;
+	mx4_pad_best<T>(l, have);
+	for (int i = tid; i < (have > k ? have : k); i += T) {
 		mx4_key key = 0;
 		int at = i;
 		if (i < have) {
-			key = best[i];
-			at = 0;
-			for (int j = 0; j < have; j++) at += best[j] > key ? 1 : 0;
+			key = l.best[i];
+			at = mx4_rank(l, have, key);
+			if (at >= k) continue;
 		}
 		if (o.keys) {
-			if (i < have) o.keys[q * stride + at] = key;
+			if (i < have) o.keys[q * kMx4ScanMaxK + at] = key;
 			if (i < have && at == k - 1) o.bound[q] = key;
 		} else {
 			o.ids[q * k + at] = i < have ? mx4_key_id(key) : -1;
@@ -180,40 +263,44 @@ __device__ void mx4_block_topk(F key_at, int m, int k, int64_t q, int64_t stride
 	}
 	if (tid == 0) {
 		if (o.keys) {
-			o.fill[q] = have;
-			if (have < k) o.bound[q] = 0;
+			o.fill[q] = out;
+			if (out < k) o.bound[q] = 0;
 		} else {
-			o.count[q] = have;
+			o.count[q] = out;
 		}
 	}
 }
-
-// one workgroup per query: the best k of level 0's products (m of them, product j belongs to row (j / 64) * 64 * step + j % 64)
-__global__ __launch_bounds__(256) void mx4_pick_first_kernel(const float *scores, int m, int64_t step, int n, int k, const uint32_t *allow, Mx4Out o,
-                                                             int64_t stride, int32_t *over)
+// The best k of them, or fewer and zeros, in any order, to k places
+template <int T>
+__device__ void mx4_block_leave(int have, int k, mx4_key *dst, Mx4PickLds &l)
 {
-	__shared__ Mx4PickLds l;
-	__shared__ mx4_key best[kMx4ScanMaxK];
-	const int64_t q = blockIdx.x;
-	const float *sc = scores + q * m;
-	auto key_at = [&](int j) -> mx4_key {
-		const int64_t id = (int64_t)(j >> 6) * 64 * step + (j & 63);
-		if (id >= n || (allow && !((allow[id >> 5] >> (id & 31)) & 1u))) return 0;
-		return mx4_make_key(sc[j], (unsigned)id);
-	};
-	if (over && threadIdx.x == 0) over[q] = 0;
-	mx4_block_topk<256>(key_at, m, k, q, stride, o, l, best);
+	const int tid = threadIdx.x & (T - 1);
+	mx4_pad_best<T>(l, have);
+	for (int i = tid; i < (have > k ? have : k); i += T) {
+		const mx4_key key = i < have ? l.best[i] : 0;
+		const int at = have > k ? mx4_rank(l, have, key) : i;
+		if (at < k) dst[at] = key;
+	}
 }
 
-// one workgroup per query: the best k of the `m` keys that the chunks left (0 = none)
+// one workgroup per query: the best k of the `m` keys that the chunks left (0 = none), 7 x 1024 at a time beside the best so far
 __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *keys, int m, int k, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
-	__shared__ mx4_key best[kMx4ScanMaxK];
 	const int64_t q = blockIdx.x;
+	const int tid = threadIdx.x;
 	const mx4_key *mine = keys + q * m;
-	auto key_at = [&](int j) -> mx4_key { return mine[j]; };
-	mx4_block_topk<1024>(key_at, m, k, q, 0, o, l, best);
+	int have = 0;
+	for (int64_t base = 0; base < m; base += 7 * 1024) {
+		mx4_key key[8];
+#pragma unroll
+		for (int j = 0; j < 7; j++) key[j] = base + j * 1024 + tid < m ? mine[base + j * 1024 + tid] : 0;
+		key[7] = tid < have ? l.best[tid] : 0;
+		__syncthreads();
+		have = mx4_block_best<1024, 8>(key, k, l);
+		__syncthreads();
+	}
+	mx4_block_put<1024>(have, k, q, o, l);
 }
 
 // one workgroup per query: the best k of what it had and of its lists
@@ -224,17 +311,21 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
                                                        int k, Mx4Out o, int32_t *over)
 {
 	__shared__ Mx4PickLds l;
-	__shared__ mx4_key best[kMx4ScanMaxK], keys[kMx4Gather];
+	__shared__ mx4_key keys[kMx4Gather];
 	__shared__ int total, lost;
 	const int64_t q = blockIdx.x;
-	const int tid = threadIdx.x, had = nbefore[q];
+	const int tid = threadIdx.x;
+	const mx4_key old = tid < kMx4ScanMaxK ? before[q * kMx4ScanMaxK + tid] : 0;  // (loads that wait for nothing: most lists hold none, one or two)
+	const int had = nbefore[q];
 	if (tid == 0) {
 		total = had;
 		lost = 0;
 	}
-	for (int i = tid; i < had; i += 256) keys[i] = before[q * kMx4ScanMaxK + i];
 	__syncthreads();
+	if (tid < had) keys[tid] = old;
 	for (int i = tid; i < parts; i += 256) {
+		const mx4_key *src = lists + (q * parts + i) * kMx4List;
+		const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(src);
 		int c = counts[q * parts + i];
 		if (c > 0) {
 			if (c > kMx4List) {
@@ -242,16 +333,20 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 				c = kMx4List;
 			}
 			const int at = atomicAdd(&total, c);
-			const mx4_key *src = lists + (q * parts + i) * kMx4List;
-			for (int j = 0; j < c; j++)
+			if (at < kMx4Gather) keys[at] = two.x;
+			if (c > 1 && at + 1 < kMx4Gather) keys[at + 1] = two.y;
+			for (int j = 2; j < c; j++)
 				if (at + j < kMx4Gather) keys[at + j] = src[j];
 		}
 	}
 	__syncthreads();
 	const int m = total < kMx4Gather ? total : kMx4Gather;
 	if (tid == 0 && (lost || total > kMx4Gather)) over[q] = 1;
-	auto key_at = [&](int j) -> mx4_key { return keys[j]; };
-	mx4_block_topk<256>(key_at, m, k, q, kMx4ScanMaxK, o, l, best);
+	mx4_key key[kMx4Gather / 256];
+#pragma unroll
+	for (int j = 0; j < kMx4Gather / 256; j++) key[j] = j * 256 + tid < m ? keys[j * 256 + tid] : 0;
+	const int have = mx4_block_best<256, kMx4Gather / 256>(key, k, l);
+	mx4_block_put<256>(have, k, q, o, l);
 }
 
 // ---------------------------------------------------------------------------------------------- products of 32 rows
@@ -277,28 +372,35 @@ __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS>
 }
 
 // ---------------------------------------------------------------------------------------------- chunks
-constexpr int kMx4ChunkQ = 8;        // queries a launch, at most
+constexpr int kMx4ChunkQ = 8;        // queries of a workgroup
 constexpr int kMx4ChunkRows = 2048;  // rows a workgroup, at most
 
 constexpr int kMx4ChunkThreads = 512;
+static_assert(kMx4ChunkThreads / 64 >= kMx4ChunkQ, "a wave for each query");
 
 // A wave takes 32 rows at a time, the next ones on their way meanwhile.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
 // quarters of the matrix work is for nothing: it is a few us at a million rows, against the reading of them.
 template <int KS>
 __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int k, int chunk,
-                                                                     const uint32_t *allow, mx4_key *out, int64_t stride)
+                                                                     const uint32_t *allow, mx4_key *out, int64_t stride, int64_t step, Mx4Out o,
+                                                                     int32_t *over, int qper)
 {
-	extern __shared__ float sc[];  // [nq][chunk]
-	__shared__ Mx4PickLds l;
+	extern __shared__ __attribute__((aligned(16))) float sc[];  // [nq][chunk]
+	__shared__ Mx4PickLds l[kMx4ChunkQ];
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, r32 = lane & 31;
 	const int64_t first = (int64_t)blockIdx.x * chunk;
-	const int m = (int)(n - first < chunk ? n - first : chunk);
-	const uint8_t *base = rows + first * row_bytes;
+	const int64_t end = step > 1 ? chunk : n - first;  // (tiles apart: the host gives as many as there are, the last may end early)
+	const int m = (int)(end < chunk ? end : chunk);
+	const int qbase = blockIdx.y * qper;
+	q += (int64_t)qbase * row_bytes;
+	nq = nq - qbase < qper ? nq - qbase : qper;
+	// row of place t: rows in a run, or (step > 1, one workgroup for them all) the 64-row tiles that are multiples of step
+	auto row_of = [&](int t) -> int64_t { return first + t + (int64_t)(t & ~63) * (step - 1); };
 	Mx4Frag<KS> b[1], f0, f1;
 	auto load = [&](int t, Mx4Frag<KS> &f) {
-		const int r = t + r32 < m ? t + r32 : m - 1;
-		mx4_load_frag<KS>(f, base + (int64_t)r * row_bytes, half);
+		const int64_t r = row_of(t + r32 < m ? t + r32 : m - 1);
+		mx4_load_frag<KS>(f, rows + (r < n ? r : n - 1) * row_bytes, half);
 	};
 	auto use = [&](int t, Mx4Frag<KS> &f) {
 		mx4_shift_scales(f, half);
@@ -337,29 +439,38 @@ __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8
 		t += STEP;
 	}
 	__syncthreads();
-	for (int qi = 0; qi < nq; qi++) {
-		auto key_at = [&](int j) -> mx4_key {
-			const int64_t id = first + j;
-			if (allow && !((allow[id >> 5] >> (id & 31)) & 1u)) return 0;
-			return mx4_make_key(sc[qi * chunk + j], (unsigned)id);
-		};
-		const mx4_key kth = mx4_block_kth<kMx4ChunkThreads>(key_at, m, k, l);
-		mx4_key *o = out + qi * stride + (int64_t)blockIdx.x * k;
-		if (tid == 0) l.pick = 0;
-		__syncthreads();
-		for (int j = tid; j < m; j += kMx4ChunkThreads) {
-			const mx4_key key = key_at(j);
-			if (key >= kth) o[atomicAdd(&l.pick, 1)] = key;
+	// One query at a time by the workgroup, or a query a wave: the first takes the less time for one or two, the second for more.
+	auto pick = [&](auto threads, Mx4PickLds &l, int qi) {
+		constexpr int T = decltype(threads)::value, N = kMx4ChunkRows / T;
+		mx4_key key[N];
+#pragma unroll
+		for (int j = 0; j < N; j++) {
+			const int at = j * T + (tid & (T - 1));
+			key[j] = 0;
+			if (j * T >= m) continue;
+			const int64_t id = row_of(at);
+			const bool in = at < m && id < n && (!allow || ((allow[id >> 5] >> (id & 31)) & 1u));
+			key[j] = in ? mx4_make_key(sc[qi * chunk + at], (unsigned)id) : 0;
 		}
-		__syncthreads();
-		const int have = l.pick;
-		for (int j = have + tid; j < k; j += kMx4ChunkThreads) o[j] = 0;
-		__syncthreads();
+		const int have = mx4_block_best<T>(key, k, l);
+		if (out) {  // one chunk of several
+			mx4_block_leave<T>(have, k, out + (qbase + qi) * stride + (int64_t)blockIdx.x * k, l);
+		} else {
+			mx4_block_put<T>(have, k, qbase + qi, o, l);
+			if (over && (tid & (T - 1)) == 0) over[qbase + qi] = 0;
+		}
+		mx4_sync<T>();
+	};
+	if (nq <= 2) {
+		for (int qi = 0; qi < nq; qi++) pick(std::integral_constant<int, kMx4ChunkThreads>{}, l[0], qi);
+	} else if (wave < nq) {
+		pick(std::integral_constant<int, 64>{}, l[wave], wave);
 	}
 }
 
 // ---------------------------------------------------------------------------------------------- levels
 constexpr int kMx4FirstTiles = 16;  // 64-row tiles of level 0, at most
+static_assert(kMx4FirstTiles * 64 <= kMx4ChunkRows, "level 0 is one chunk");
 
 struct Mx4Level {
 	const uint8_t *q, *rows;
@@ -699,7 +810,7 @@ template <int KS>
 __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, const int32_t *over, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
-	__shared__ mx4_key keys[kMx4Gather], best[kMx4ScanMaxK];
+	__shared__ mx4_key keys[kMx4Gather];
 	__shared__ int count;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, r32 = lane & 31;
 	for (int q = blockIdx.x; q < a.nq; q += gridDim.x) {
@@ -707,7 +818,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 		Mx4Frag<KS> b[1];
 		mx4_load_frag<KS>(b[0], a.q + (int64_t)q * mx4_row_bytes(64 * KS), half);
 		mx4_shift_scales(b[0], half);
-		mx4_key kth = 1;  // keys below it are not wanted
+		int have = 0;
 		if (tid == 0) count = 0;
 		__syncthreads();
 		for (int64_t base = 0; base < a.n; base += 128) {
@@ -725,31 +836,24 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 						const int64_t id = row0 + 8 * (i >> 2) + 4 * half + (i & 3);
 						if (id < a.n && (!a.allow || ((a.allow[id >> 5] >> (id & 31)) & 1u))) {
 							const mx4_key key = mx4_make_key(acc[0][i], (unsigned)id);
-							if (key >= kth) keys[atomicAdd(&count, 1)] = key;
+							if (key) keys[atomicAdd(&count, 1)] = key;
 						}
 					}
 				}
 			}
 			__syncthreads();
-			const int have = count;
-			if (have > kMx4Gather - 128) {
-				auto key_at = [&](int j) -> mx4_key { return keys[j]; };
-				kth = mx4_block_kth<256>(key_at, have, k, l);
-				if (tid == 0) l.pick = 0;
+			if (count > kMx4Gather - 128 || base + 128 >= a.n) {  // cut to the best
+				mx4_key key[kMx4Gather / 256];
+#pragma unroll
+				for (int j = 0; j < kMx4Gather / 256; j++) key[j] = j * 256 + tid < count ? keys[j * 256 + tid] : 0;
 				__syncthreads();
-				for (int j = tid; j < have; j += 256)
-					if (keys[j] >= kth) best[atomicAdd(&l.pick, 1)] = keys[j];
-				__syncthreads();
-				const int m = l.pick;
-				for (int j = tid; j < m; j += 256) keys[j] = best[j];
-				if (tid == 0) count = m;
+				have = mx4_block_best<256>(key, k, l);
+				for (int j = tid; j < have; j += 256) keys[j] = l.best[j];
+				if (tid == 0) count = have;
 			}
 			__syncthreads();
 		}
-		auto key_at = [&](int j) -> mx4_key { return keys[j]; };
-		const int have = count;
-		__syncthreads();
-		mx4_block_topk<256>(key_at, have, k, q, 0, o, l, best);
+		mx4_block_put<256>(have, k, q, o, l);
 		__syncthreads();
 	}
 }
@@ -758,10 +862,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 constexpr int kMx4SlabQ = 8192;       // queries that are dealt with at a time
 constexpr int kMx4StreamGroups = 4;   // up to so many groups of 64 queries: mx4_stream_kernel, more: mx4_stage_kernel
 constexpr int kMx4StreamWaves = 2048;
-#ifndef MX4_R
-#define MX4_R 10
-#endif
-constexpr int kMx4MostRatio = MX4_R;
+constexpr int kMx4MostRatio = 10;  // (4 to 14 are within 3 % of each other but for the launches they save)
 
 struct Mx4Plan {
 	bool chunks;
@@ -816,8 +917,7 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 1) : most_waves);
 	}
 	p.parts = 2 * p.splits;
-	p.ws = mx4_up((size_t)p.slab * kMx4ScanMaxK * 8) + mx4_up((size_t)p.slab * 8) + 2 * mx4_up((size_t)p.slab * 4) +
-	       mx4_up((size_t)p.slab * p.first_rows * 4 + 4);
+	p.ws = mx4_up((size_t)p.slab * kMx4ScanMaxK * 8) + mx4_up((size_t)p.slab * 8) + 2 * mx4_up((size_t)p.slab * 4);
 	if (p.levels) p.ws += mx4_up((size_t)p.slab * p.parts * 4) + mx4_up((size_t)p.slab * p.parts * kMx4List * 8);
 	return p;
 }
@@ -850,7 +950,8 @@ hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const hipError_t e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, 0>::set);
 	if (e != hipSuccess) return e;
 	if (p.parts > 0)
-		hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(p.parts), dim3(kMx4ChunkThreads), lds, s, q, nq, rows, n, k, p.chunk, allow, keys, stride);
+		hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(p.parts, 1), dim3(kMx4ChunkThreads), lds, s, q, nq, rows, n, k, p.chunk, allow, keys, stride, (int64_t)1, Mx4Out{},
+		                   static_cast<int32_t *>(nullptr), kMx4ChunkQ);
 	hipLaunchKernelGGL(mx4_pick_chunks_kernel, dim3(nq), dim3(1024), 0, s, keys, (int)stride, k, o);
 	return hipGetLastError();
 }
@@ -870,8 +971,6 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	mx4_key *bound = static_cast<mx4_key *>(take((size_t)p.slab * 8));
 	int32_t *nbest = static_cast<int32_t *>(take((size_t)p.slab * 4));
 	int32_t *over = static_cast<int32_t *>(take((size_t)p.slab * 4));
-	const int m = p.first_rows;
-	float *scores = static_cast<float *>(take((size_t)p.slab * m * 4 + 4));
 	Mx4Level a{};
 	a.q = q;
 	a.rows = rows;
@@ -892,9 +991,13 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	if (p.levels && stage)
 		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS>), (int)lds,
 		                  Mx4Mark<KS, 1>::set);
-	if (e == hipSuccess) e = mx4_launch_product_tiles(q, nq, rows, n, m, p.step0, KS, row_bytes, scores, m, s);
+	if (e == hipSuccess)
+		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, 0>::set);
 	if (e != hipSuccess) return e;
-	hipLaunchKernelGGL(mx4_pick_first_kernel, dim3(nq), dim3(256), 0, s, scores, m, p.step0, n, k, allow, p.levels ? mid : last, (int64_t)kMx4ScanMaxK, over);
+	const int qper = nq >= 256 * kMx4ChunkQ ? kMx4ChunkQ : (nq + 255) / 256;  // a workgroup for every compute unit if there are queries enough
+	hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(1, (nq + qper - 1) / qper), dim3(kMx4ChunkThreads),
+	                   (size_t)qper * (p.first_rows ? p.first_rows : 64) * 4, s, q, nq, rows, n, k, p.first_rows, allow,
+	                   static_cast<mx4_key *>(nullptr), (int64_t)0, p.step0, p.levels ? mid : last, over, qper);
 	const int64_t tiles = ((int64_t)n + 63) / 64;
 	a.step = p.step0;
 	a.skip = p.ratio > 1 ? (unsigned)((((uint64_t)1 << 32) + p.ratio - 2) / (p.ratio - 1)) : 0;
