@@ -303,29 +303,40 @@ __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *ke
 	mx4_block_put<1024>(have, k, q, o, l);
 }
 
-// one workgroup per query: the best k of what it had and of its lists
+// T threads per query (a workgroup, or a wave of one): the best k of what it had and of its lists, CAP keys in all
 constexpr int kMx4List = 64;       // keys of a list
 constexpr int kMx4Gather = 2048;   // keys of all lists of a query
+constexpr int kMx4GatherFew = 512;  // where no more are expected
 
+template <int T, int CAP>
 __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, const int32_t *counts, int parts, const mx4_key *before, const int32_t *nbefore,
-                                                       int k, Mx4Out o, int32_t *over)
+                                                       int nq, int k, Mx4Out o, int32_t *over)
 {
-	__shared__ Mx4PickLds l;
-	__shared__ mx4_key keys[kMx4Gather];
-	__shared__ int total, lost;
-	const int64_t q = blockIdx.x;
-	const int tid = threadIdx.x;
-	const mx4_key old = tid < kMx4ScanMaxK ? before[q * kMx4ScanMaxK + tid] : 0;  // (loads that wait for nothing: most lists hold none, one or two)
+	__shared__ Mx4PickLds ls[256 / T];
+	__shared__ __attribute__((aligned(16))) mx4_key keyss[256 / T][CAP];
+	__shared__ int totals[256 / T], losts[256 / T];
+	const int tid = threadIdx.x & (T - 1), me = threadIdx.x / T;
+	const int64_t q = (int64_t)blockIdx.x * (256 / T) + me;
+	if (q >= nq) return;  // (T = 256: never; T = 64: whole waves, which share nothing)
+	Mx4PickLds &l = ls[me];
+	mx4_key *keys = keyss[me];
+	int &total = totals[me], &lost = losts[me];
+	mx4_key old[(kMx4ScanMaxK + T - 1) / T];  // loads that wait for nothing
+#pragma unroll
+	for (int j = 0; j < (kMx4ScanMaxK + T - 1) / T; j++) old[j] = j * T + tid < kMx4ScanMaxK ? before[q * kMx4ScanMaxK + j * T + tid] : 0;
 	const int had = nbefore[q];
 	if (tid == 0) {
 		total = had;
 		lost = 0;
 	}
-	__syncthreads();
-	if (tid < had) keys[tid] = old;
-	for (int i = tid; i < parts; i += 256) {
+	mx4_sync<T>();
+#pragma unroll
+	for (int j = 0; j < (kMx4ScanMaxK + T - 1) / T; j++)
+		if (j * T + tid < had) keys[j * T + tid] = old[j];
+#pragma unroll 4
+	for (int i = tid; i < parts; i += T) {
 		const mx4_key *src = lists + (q * parts + i) * kMx4List;
-		const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(src);
+		const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(src);  // most lists hold none, one or two
 		int c = counts[q * parts + i];
 		if (c > 0) {
 			if (c > kMx4List) {
@@ -333,20 +344,20 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 				c = kMx4List;
 			}
 			const int at = atomicAdd(&total, c);
-			if (at < kMx4Gather) keys[at] = two.x;
-			if (c > 1 && at + 1 < kMx4Gather) keys[at + 1] = two.y;
+			if (at < CAP) keys[at] = two.x;
+			if (c > 1 && at + 1 < CAP) keys[at + 1] = two.y;
 			for (int j = 2; j < c; j++)
-				if (at + j < kMx4Gather) keys[at + j] = src[j];
+				if (at + j < CAP) keys[at + j] = src[j];
 		}
 	}
-	__syncthreads();
-	const int m = total < kMx4Gather ? total : kMx4Gather;
-	if (tid == 0 && (lost || total > kMx4Gather)) over[q] = 1;
-	mx4_key key[kMx4Gather / 256];
+	mx4_sync<T>();
+	const int m = total < CAP ? total : CAP;
+	if (tid == 0 && (lost || total > CAP)) over[q] = 1;
+	mx4_key key[CAP / T];
 #pragma unroll
-	for (int j = 0; j < kMx4Gather / 256; j++) key[j] = j * 256 + tid < m ? keys[j * 256 + tid] : 0;
-	const int have = mx4_block_best<256, kMx4Gather / 256>(key, k, l);
-	mx4_block_put<256>(have, k, q, o, l);
+	for (int j = 0; j < CAP / T; j++) key[j] = j * T + tid < m ? keys[j * T + tid] : 0;
+	const int have = mx4_block_best<T>(key, k, l);
+	mx4_block_put<T>(have, k, q, o, l);
 }
 
 // ---------------------------------------------------------------------------------------------- products of 32 rows
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8
 }
 
 // ---------------------------------------------------------------------------------------------- levels
-constexpr int kMx4FirstTiles = 16;  // 64-row tiles of level 0, at most
+constexpr int kMx4FirstTiles = 32;  // 64-row tiles of level 0, at most
 static_assert(kMx4FirstTiles * 64 <= kMx4ChunkRows, "level 0 is one chunk");
 
 struct Mx4Level {
@@ -477,7 +488,7 @@ struct Mx4Level {
 	const uint32_t *allow;
 	int nq, n;
 	int64_t step;     // see mx4_level_tile
-	unsigned skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
+	uint64_t skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
 	int tiles;
 	const mx4_key *bound;  // [nq], 0 = none
 	mx4_key *lists;   // [nq][parts][kMx4List]
@@ -488,7 +499,7 @@ struct Mx4Level {
 // tile i of a level, first row: i / (ratio - 1) by a multiplication, exact for i (ratio - 1) < 2^32 (i < 2^25)
 __device__ __forceinline__ int64_t mx4_tile_row(const Mx4Level &a, unsigned i)
 {
-	if (a.skip) i += (unsigned)(((uint64_t)i * a.skip) >> 32) + 1;
+	if (a.skip) i += (unsigned)((i * a.skip) >> 32) + 1;
 	return (int64_t)i * a.step * 64;
 }
 
@@ -505,7 +516,7 @@ struct Mx4Queries {
 	Mx4Frag<KS> b[C];
 	float bound[C];
 	mx4_key bkey[C];
-	unsigned list[C];  // index of the list's first key
+	unsigned list[C];  // byte offset of the list's first key (262 144 lists at most: mx4_plan)
 	int count[C];
 };
 
@@ -520,7 +531,7 @@ __device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS, C> &w, const Mx4
 		w.bkey[c] = a.bound[qs];
 		// no query in this column: nothing is >= NaN
 		w.bound[c] = q >= a.nq ? __uint_as_float(0x7fc00000u) : w.bkey[c] ? mx4_key_value(w.bkey[c]) : -__builtin_inff();
-		w.list[c] = ((unsigned)qs * a.parts + part) * kMx4List;
+		w.list[c] = ((unsigned)qs * a.parts + part) * (kMx4List * 8);
 		w.count[c] = 0;
 	}
 }
@@ -551,6 +562,7 @@ __device__ __forceinline__ bool mx4_test(const Mx4Queries<KS, C> &w, const mx4_v
 template <int KS, int C>
 __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], const float (&m)[C][4], int64_t row0, int half)
 {
+	char *lists = reinterpret_cast<char *>(a.lists);
 	unsigned id0 = (unsigned)row0 + 4 * half;
 	asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
 #pragma unroll
@@ -561,10 +573,13 @@ __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level 
 #pragma unroll
 				for (int j = 0; j < 4; j++) {
 					const float v = acc[c][4 * g + j];
-					if (v >= w.bound[c]) {
-						const mx4_key key = mx4_make_key(v, id0 + 8 * g + j);
-						if (key > w.bkey[c]) {
-							if (w.count[c] < kMx4List) a.lists[(size_t)w.list[c] + w.count[c]] = key;
+					if (__ballot(v >= w.bound[c])) {
+						const unsigned b = __float_as_uint(v + 0.f);  // mx4_make_key of a number
+						const mx4_key key = ((mx4_key)(b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) << 32) | ~(id0 + 8 * g + j);
+						if (v >= w.bound[c] && key > w.bkey[c]) {
+							// (a list that is full loses its last key, and says so by its count)
+							const unsigned at = w.list[c] + 8u * (unsigned)(w.count[c] < kMx4List ? w.count[c] : kMx4List - 1);
+							*reinterpret_cast<mx4_key *>(lists + at) = key;
 							w.count[c]++;
 						}
 					}
@@ -641,37 +656,18 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 	mx4_store_counts(w, a, group * 32 * C, 2 * first + half, r32);
 }
 
-// 64 consecutive rows a tile, staged in LDS for up to 8 waves of 64 queries each.  The tiles come by LDS-DMA into a ring of four, three tiles
-// ahead; one barrier a tile: after it tile t + 1 is there for everybody and the place of tile t - 1 is free.  An image row is the packed
-// row, plus one slot of 16 bytes where that makes the stride an odd number of slots: then the 16 lanes that an LDS read serves at a time hit
-// 16 different slots.  Two waves a SIMD: one tests while the other multiplies.
-constexpr int kMx4Ring = 4;
+// Tiles of 64 rows, staged in LDS for up to 8 waves of 64 queries each.  Groups of tiles come by LDS-DMA into two places in turn: while one group is
+// worked on the tiles of the next are asked for, one after the other.  One barrier a group: a wave that appends keeps the others waiting there, the
+// less the further the barriers are apart (4096 queries, 900 000 x 512, 168 candidates a query: barriers 1 tile apart 960 us, 2 tiles 880 us).
+// An image row is the packed row, plus one slot of 16 bytes where that makes the stride an odd number of slots: then the 16 lanes that an LDS read
+// serves at a time hit 16 different slots.  Two waves a SIMD.
 static __device__ __align__(16) int g_mx4_nan[4] = {-1, -1, -1, -1};  // scales 255: the blocks of a row that is left out
 
 __host__ __device__ constexpr int mx4_image_slots(int row_bytes) { return (row_bytes / 16) | 1; }
 
-// Tiles between two barriers, as many as the ring has room for: a wave that appends keeps the others waiting at the barrier, the less the further
-// these are apart (4096 queries, 900 000 x 512, 168 candidates a query: 1 tile 960 us, 2 tiles 880 us).
-__host__ __device__ constexpr int mx4_stage_group(int ks) { return ks <= 4 ? 4 : ks <= 8 ? 2 : 1; }
-
-template <int N>
-__device__ __forceinline__ void mx4_wait_vm()
-{
-	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// until at most n vector-memory operations of this wave are outstanding (n is wave-uniform); more than MOST counts as 0
-template <int MOST = 12>
-__device__ __forceinline__ void mx4_wait_vm_upto(int n)
-{
-	if constexpr (MOST == 0) {
-		mx4_wait_vm<0>();
-	} else {
-		if (n == MOST)
-			mx4_wait_vm<MOST>();
-		else
-			mx4_wait_vm_upto<MOST - 1>(n);
-	}
-}
+// tiles of a group (a power of two): as many as LDS has room for twice
+__host__ __device__ constexpr int mx4_stage_group(int ks) { return ks <= 8 ? 4 : 2; }
+__host__ __device__ constexpr size_t mx4_stage_lds(int ks) { return (size_t)2 * mx4_stage_group(ks) * mx4_image_slots(mx4_row_bytes(64 * ks)) * 1024; }
 
 template <int KS>
 __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtiles, int splits)
@@ -685,6 +681,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	const int slots = row_bytes / 16, islots = slots | 1;
 	const int tile_bytes = islots * 64 * 16;
+	constexpr int G = mx4_stage_group(KS);
 	const int q0 = (qtile * nwaves + wave) * 64;
 	Mx4Queries<KS, 2> w;
 	mx4_load_queries(w, a, q0, 2 * split + half, half, r32);
@@ -696,7 +693,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	auto fetch = [&](int t) {
 		const int64_t row0 = mx4_tile_row(a, split + t * splits);
 		const uint8_t *base = a.rows + row0 * row_bytes;
-		unsigned char *dst = lds + (t & (kMx4Ring * mx4_stage_group(KS) - 1)) * tile_bytes;
+		unsigned char *dst = lds + (t & (2 * G - 1)) * tile_bytes;
 		if (islots == slots && !a.allow && row0 + 64 <= a.n) {  // the image is the tile as it lies in memory
 			for (int i = wave; i < islots; i += nwaves)
 				__builtin_amdgcn_global_load_lds((glb_ptr_t)(base + i * 1024 + (unsigned)lane * 16), (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
@@ -717,17 +714,10 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 			__builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
 		}
 	};
-	const int mine = (islots - wave + nwaves - 1) / nwaves;  // instructions of a fetch by this wave
-	constexpr int G = mx4_stage_group(KS);
-	auto image = [&](int t, int h) -> const unsigned char * { return lds + (t & (kMx4Ring * G - 1)) * tile_bytes + (h * 32 + r32) * islots * 16; };
-	mx4_wait_vm<0>();
-	for (int t = 0; t < 3 * G && t < ntiles; t++) fetch(t);
-	mx4_wait_vm_upto(0);  // (once)
-	__builtin_amdgcn_s_barrier();
-	asm volatile("" ::: "memory");
+	auto image = [&](int t, int h) -> const unsigned char * { return lds + (t & (2 * G - 1)) * tile_bytes + (h * 32 + r32) * islots * 16; };
+	for (int t = 0; t < G && t < ntiles; t++) fetch(t);
 	constexpr bool AHEAD = KS <= 8;  // room in the registers for the fragments of the next 32 rows
 	Mx4Frag<KS> f0, f1;
-	if (AHEAD && ntiles > 0) mx4_load_frag<KS>(f0, image(0, 0), half);
 	constexpr bool PIPED = KS <= 12;
 	// Two sets of accumulators (where there is room): the products of one 32 rows are tested while those of the next are computed.
 	mx4_v16f accA[2], accB[2];
@@ -770,26 +760,23 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append(w, a, then, m, row, half);
 	};
 	for (int t = 0; t < ntiles; t += G) {
-		// this wave's share of the next G tiles is there (loads complete in order; the G after them may be under way) ...
-		mx4_wait_vm_upto(t + 3 * G <= ntiles ? G * mine : 0);
-		__builtin_amdgcn_s_barrier();  // ... and everybody's, and the G before these are done with
+		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the group is there ...
+		__builtin_amdgcn_s_barrier();                     // ... and everybody's, and the group before it is done with
 		asm volatile("" ::: "memory");
-#pragma unroll
-		for (int g = 0; g < G; g++)
-			if (t + 3 * G + g < ntiles) fetch(t + 3 * G + g);
-#pragma unroll
-		for (int g = 0; g < G; g++) {
-			if (g > 0 && t + g >= ntiles) break;
-			const int64_t row0 = mx4_tile_row(a, split + (t + g) * splits);
-			if (!AHEAD) mx4_load_frag<KS>(f0, image(t + g, 0), half);
+		if (AHEAD) mx4_load_frag<KS>(f0, image(t, 0), half);
+#pragma unroll 2
+		for (int u = t; u < t + G && u < ntiles; u++) {
+			if (u + G < ntiles) fetch(u + G);
+			const int64_t row0 = mx4_tile_row(a, split + u * splits);
+			if (!AHEAD) mx4_load_frag<KS>(f0, image(u, 0), half);
 			if (AHEAD) {
-				mx4_load_frag<KS>(f1, image(t + g, 1), half);
+				mx4_load_frag<KS>(f1, image(u, 1), half);
 				__builtin_amdgcn_sched_barrier(0);
 			}
 			step(f0, accA, accB, PIPED ? rowB : row0);
-			if (!AHEAD) mx4_load_frag<KS>(f1, image(t + g, 1), half);
-			if (AHEAD && t + g + 1 < ntiles) {
-				mx4_load_frag<KS>(f0, image(t + g + 1, 0), half);
+			if (!AHEAD) mx4_load_frag<KS>(f1, image(u, 1), half);
+			if (AHEAD) {
+				mx4_load_frag<KS>(f0, image(u + 1, 0), half);  // (behind the group's last tile: never used)
 				__builtin_amdgcn_sched_barrier(0);
 			}
 			step(f1, PIPED ? accB : accA, accA, PIPED ? row0 : row0 + 32);
@@ -865,7 +852,7 @@ constexpr int kMx4StreamWaves = 2048;
 constexpr int kMx4MostRatio = 10;  // (4 to 14 are within 3 % of each other but for the launches they save)
 
 struct Mx4Plan {
-	bool chunks;
+	bool chunks, few;  // few: keys that a query gathers in a level
 	int chunk, parts;  // chunks: rows of one, how many; levels: lists of a query
 	int levels, ratio, first_rows;  // levels after level 0; rows of level 0 (a multiple of 64)
 	int64_t step0;
@@ -890,7 +877,8 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 	const int64_t tiles = ((int64_t)n + 63) / 64;
 	// About k (ratio - 1) keys are expected of a level, with a standard deviation of ratio sqrt(k): a query gathers that and 8 deviations
 	int most = kMx4MostRatio;
-	while (most > 4 && k * (most - 1) + 8 * most * (int)std::ceil(std::sqrt((double)k)) > kMx4Gather - k) most--;
+	auto gathered = [&](int ratio) { return k * ratio + 8 * ratio * (int)std::ceil(std::sqrt((double)k)); };
+	while (most > 4 && gathered(most) > kMx4Gather) most--;
 	p.levels = 0;
 	p.ratio = 0;
 	p.step0 = 1;
@@ -904,6 +892,7 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 			if (p.ratio <= most) break;
 		}
 	}
+	p.few = nq >= 2048 && gathered(p.ratio) <= kMx4GatherFew;  // (1000 queries: 7.5 us by workgroups, 10 us by waves; 4096: 23 and 12)
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
 	p.slab = nq < kMx4SlabQ ? nq : kMx4SlabQ;
 	p.qgroups = (p.slab + 63) / 64;
@@ -986,7 +975,8 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const Mx4Out mid = {nullptr, nullptr, nullptr, best, bound, nbest};
 	const bool stage = p.qtiles > 0;
 	const int nwaves = stage ? (p.qgroups + p.qtiles - 1) / p.qtiles : 0;
-	const size_t lds = (size_t)kMx4Ring * mx4_stage_group(KS) * mx4_image_slots(row_bytes) * 1024;
+	constexpr size_t lds = mx4_stage_lds(KS);
+	static_assert(lds <= 160 * 1024, "LDS of a compute unit");
 	hipError_t e = hipSuccess;
 	if (p.levels && stage)
 		e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_stage_kernel<KS>), (int)lds,
@@ -1000,7 +990,7 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	                   static_cast<mx4_key *>(nullptr), (int64_t)0, p.step0, p.levels ? mid : last, over, qper);
 	const int64_t tiles = ((int64_t)n + 63) / 64;
 	a.step = p.step0;
-	a.skip = p.ratio > 1 ? (unsigned)((((uint64_t)1 << 32) + p.ratio - 2) / (p.ratio - 1)) : 0;
+	a.skip = p.ratio > 1 ? (((uint64_t)1 << 32) + p.ratio - 2) / (p.ratio - 1) : 0;
 	for (int l = 1; l <= p.levels; l++) {
 		const int64_t before = (tiles + a.step - 1) / a.step;
 		a.step /= p.ratio;
@@ -1009,7 +999,12 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 			hipLaunchKernelGGL((mx4_stage_kernel<KS>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
 		else
 			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
-		hipLaunchKernelGGL(mx4_pick_kernel, dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, k, l < p.levels ? mid : last, over);
+		if (p.few)
+			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherFew>), dim3((nq + 3) / 4), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			                   l < p.levels ? mid : last, over);
+		else
+			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4Gather>), dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			                   l < p.levels ? mid : last, over);
 	}
 	if (p.levels)
 		hipLaunchKernelGGL((mx4_rescue_kernel<KS>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
