@@ -849,7 +849,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 constexpr int kMx4SlabQ = 8192;       // queries that are dealt with at a time
 constexpr int kMx4StreamGroups = 4;   // up to so many groups of 64 queries: mx4_stream_kernel, more: mx4_stage_kernel
 constexpr int kMx4StreamWaves = 2048;
-constexpr int kMx4MostRatio = 10;  // (4 to 14 are within 3 % of each other but for the launches they save)
+constexpr int kMx4MostRatio = 10, kMx4MostRatioFew = 64;  // many queries: 4 to 14 are within 3 %; few: a candidate costs little against a launch
 
 struct Mx4Plan {
 	bool chunks, few;  // few: keys that a query gathers in a level
@@ -874,10 +874,13 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 		p.ws = mx4_up((size_t)nq * p.parts * k * 8 + 8);
 		return p;
 	}
+	p.slab = nq < kMx4SlabQ ? nq : kMx4SlabQ;
+	p.qgroups = (p.slab + 63) / 64;
 	const int64_t tiles = ((int64_t)n + 63) / 64;
-	// About k (ratio - 1) keys are expected of a level, with a standard deviation of ratio sqrt(k): a query gathers that and 8 deviations
-	int most = kMx4MostRatio;
-	auto gathered = [&](int ratio) { return k * ratio + 8 * ratio * (int)std::ceil(std::sqrt((double)k)); };
+	// The rows of a level that beat the bound are about ratio x Gamma(k) in number, if the levels are alike: more than ratio (k + 6 sqrt(k) + 12)
+	// about once in 10^9 queries, and that many a query can gather
+	int most = p.qgroups > kMx4StreamGroups ? kMx4MostRatio : kMx4MostRatioFew;
+	auto gathered = [&](int ratio) { return ratio * (k + 6 * std::sqrt((double)k) + 12); };
 	while (most > 4 && gathered(most) > kMx4Gather) most--;
 	p.levels = 0;
 	p.ratio = 0;
@@ -894,8 +897,6 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 	}
 	p.few = nq >= 2048 && gathered(p.ratio) <= kMx4GatherFew;  // (1000 queries: 7.5 us by workgroups, 10 us by waves; 4096: 23 and 12)
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
-	p.slab = nq < kMx4SlabQ ? nq : kMx4SlabQ;
-	p.qgroups = (p.slab + 63) / 64;
 	if (p.qgroups > kMx4StreamGroups) {  // (groups of 64)
 		p.qtiles = (p.qgroups + 7) / 8;
 		p.splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles);  // 8 x qtiles workgroups at a time: one a compute unit
