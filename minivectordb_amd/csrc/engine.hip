@@ -1926,6 +1926,7 @@ int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint
 	if (nq == 0) return 1;
 	if (!d_q || (n > 0 && !d_rows) || !d_out_ids || !d_out_val || !d_out_count || !d_ws) return mx4_fail(h, fn, "null pointer");
 	if (mx4_misaligned(d_q) || mx4_misaligned(d_rows)) return mx4_fail(h, fn, "packed rows must be 16-byte aligned");
+	if (reinterpret_cast<uintptr_t>(d_allow) % 4) return mx4_fail(h, fn, "the filter is not aligned to its type");
 	if (mx4_misaligned(d_ws)) return mx4_fail(h, fn, "the workspace must be 16-byte aligned");
 	if (ws_bytes < mx4_scan_workspace(nq, n, h->cfg.dim, k)) return mx4_fail(h, fn, "the workspace is smaller than mvdb_mx4_scan_workspace says");
 	DeviceGuard dev(h);

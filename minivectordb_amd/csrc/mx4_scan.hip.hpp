@@ -150,13 +150,13 @@ __device__ int mx4_block_best(const mx4_key (&key)[N], int k, Mx4PickLds &l)
 	}
 	const float most = mx4_key_value((mx4_key)hi << 32), least = mx4_key_value((mx4_key)~nlo << 32), span = most - least;
 	bool done = false;
-	if (hi != 0 && span > 0.f && span < 3e38f) {
+	if (hi != 0 && span > 1e-30f && span < 3e38f) {
 		const float scale = 255.f / span;  // (subtraction, product and conversion keep the order of the values)
 		int bin[N];
 #pragma unroll
 		for (int j = 0; j < N; j++) {
-			const int x = (int)((mx4_key_value(key[j]) - least) * scale);
-			bin[j] = key[j] ? (x < 255 ? x : 255) : -1;
+			const float x = key[j] ? (mx4_key_value(key[j]) - least) * scale : -1.f;
+			bin[j] = x < 255.f ? (int)x : 255;
 			if (bin[j] >= 0) atomicAdd(&l.hist[bin[j]], 1);
 		}
 		mx4_sync<T>();
@@ -305,8 +305,10 @@ __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *ke
 
 // T threads per query (a workgroup, or a wave of one): the best k of what it had and of its lists, CAP keys in all
 constexpr int kMx4List = 64;       // keys of a list
-constexpr int kMx4Gather = 2048;   // keys of all lists of a query
-constexpr int kMx4GatherFew = 512;  // where no more are expected
+// Keys of all lists of a query.  The plan sees to it that a random order of the rows stays far below them; what asks for more is a run of neighbouring
+// rows that are all candidates and that the levels before have missed, at most 64 x ratio of them.
+constexpr int kMx4Gather = 2048, kMx4GatherFewQueries = 4096;
+constexpr int kMx4GatherWave = 768;  // the most that a wave deals with
 
 template <int T, int CAP>
 __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, const int32_t *counts, int parts, const mx4_key *before, const int32_t *nbefore,
@@ -849,7 +851,7 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 constexpr int kMx4SlabQ = 8192;       // queries that are dealt with at a time
 constexpr int kMx4StreamGroups = 4;   // up to so many groups of 64 queries: mx4_stream_kernel, more: mx4_stage_kernel
 constexpr int kMx4StreamWaves = 2048;
-constexpr int kMx4MostRatio = 10, kMx4MostRatioFew = 64;  // many queries: 4 to 14 are within 3 %; few: a candidate costs little against a launch
+constexpr int kMx4MostRatio = 10, kMx4MostRatioFew = 52;  // many queries: 4 to 14 are within 3 %; few: a candidate costs little against a launch
 
 struct Mx4Plan {
 	bool chunks, few;  // few: keys that a query gathers in a level
@@ -879,7 +881,8 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 	const int64_t tiles = ((int64_t)n + 63) / 64;
 	// The rows of a level that beat the bound are about ratio x Gamma(k) in number, if the levels are alike: more than ratio (k + 6 sqrt(k) + 12)
 	// about once in 10^9 queries, and that many a query can gather
-	int most = p.qgroups > kMx4StreamGroups ? kMx4MostRatio : kMx4MostRatioFew;
+	const bool many = p.qgroups > kMx4StreamGroups;
+	int most = many ? kMx4MostRatio : kMx4MostRatioFew;
 	auto gathered = [&](int ratio) { return ratio * (k + 6 * std::sqrt((double)k) + 12); };
 	while (most > 4 && gathered(most) > kMx4Gather) most--;
 	p.levels = 0;
@@ -895,9 +898,9 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 			if (p.ratio <= most) break;
 		}
 	}
-	p.few = nq >= 2048 && gathered(p.ratio) <= kMx4GatherFew;  // (1000 queries: 7.5 us by workgroups, 10 us by waves; 4096: 23 and 12)
+	p.few = nq >= 2048 && gathered(p.ratio) <= kMx4GatherWave - 256;  // (1000 queries: 7.5 us by workgroups, 10 us by waves; 4096: 23 and 12)
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
-	if (p.qgroups > kMx4StreamGroups) {  // (groups of 64)
+	if (many) {
 		p.qtiles = (p.qgroups + 7) / 8;
 		p.splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles);  // 8 x qtiles workgroups at a time: one a compute unit
 	} else {
@@ -1001,7 +1004,10 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 		else
 			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
 		if (p.few)
-			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherFew>), dim3((nq + 3) / 4), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherWave>), dim3((nq + 3) / 4), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			                   l < p.levels ? mid : last, over);
+		else if (!stage)
+			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4GatherFewQueries>), dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
 			                   l < p.levels ? mid : last, over);
 		else
 			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4Gather>), dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,

@@ -266,15 +266,36 @@ def test_scan_ordered_rows(engines, nq, order):
     _check_scan(engines(64), M.pack(q), r, 100)
 
 
-def test_scan_adversarial_levels(engines):
-    """More rows beat every earlier row than any buffer holds: rows in blocks of 64, most blocks good, every period-th poor."""
+@pytest.mark.parametrize("nq,k", [(12, 10), (12, 100), (300, 10), (300, 100)])
+def test_scan_adversarial_levels(engines, nq, k):
+    """Rows in blocks of 64, every period-th block poor and the others good: where the period is that of a level, every row of
+    the next beats the bound, more than any buffer holds."""
     rng = np.random.default_rng(3)
     n = 64 * 1500
-    for period in range(2, 13):
+    q = M.pack(np.ones((nq, 64)) + 0.5 * rng.integers(0, 2, (nq, 64)))
+    for period in (2, 4, 5, 6, 7, 8, 10, 47, 49):
         good = (np.arange(n) // 64) % period != 0
         x = np.where(good[:, None], 1.0, -1.0) * (1 + 0.25 * rng.integers(0, 3, (n, 64)))
-        q = M.pack(np.ones((12, 64)) + 0.5 * rng.integers(0, 2, (12, 64)))
-        _check_scan(engines(64), q, M.pack(x), 100 if period % 2 else 10)
+        _check_scan(engines(64), q, M.pack(x), k)
+
+
+def test_scan_crowded_rows(engines):
+    """Hundreds of neighbouring rows that are all candidates of one query (the chunks of one long document)."""
+    rng = np.random.default_rng(4)
+    x = _unit(rng, 50000, 64)
+    q = _unit(rng, 30, 64)
+    for i in range(30):
+        at = 1000 + 1500 * i + 37 * i
+        x[at : at + 20 * (i + 1)] = q[i] + 0.2 * rng.standard_normal((20 * (i + 1), 64)) / 8
+    for nq in (1, 5, 30):
+        _check_scan(engines(64), M.pack(q[-nq:]), M.pack(x), 128)
+    _check_scan(engines(64), M.pack(np.repeat(q, 10, 0)), M.pack(x), 50)
+
+
+def test_scan_many_queries(engines):
+    """More queries than are dealt with at a time."""
+    rng = np.random.default_rng(6)
+    _check_scan(engines(64), M.pack(_unit(rng, 8200, 64)), M.pack(_unit(rng, 3300, 64)), 3)
 
 
 @pytest.mark.parametrize("nq", [1, 70])
@@ -406,6 +427,33 @@ def test_graph_capture(engines):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(got2, want2))
             assert torch.equal(scores, mx.product(mx.quantize(x), rows[:500]))
+
+
+@pytest.mark.parametrize("nq", [1, 40, 300])
+def test_capture_without_a_call_before(gpu, nq):
+    """A handle and a row length that nothing has used yet: the first call of all may be the captured one."""
+    import torch
+    from minivectordb_amd import HipBridge
+    from minivectordb_amd.pipeline import ResidentMx4
+    dim = {1: 708, 40: 836, 300: 900}[nq]
+    b = HipBridge(device=0)
+    b.init(dict(dim=dim, m=8, ef=50, capacity=8, seed=1))
+    mx = ResidentMx4(b, torch.device("cuda", 0))
+    rng = np.random.default_rng(nq)
+    q, r = M.pack(_unit(rng, nq, dim)), M.pack(_unit(rng, 5000, dim))
+    qd, rd = _to(q), _to(r)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = mx.scan_many(qd, rd, 10)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(got[0].cpu().numpy(), M.topk(M.products(q, r, dim)[0], 10)[0])
+    del graph
+    b.close()
 
 
 def test_streams_side_by_side(engines):

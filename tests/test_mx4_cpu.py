@@ -101,6 +101,7 @@ def test_device_entry_points_refuse():
     _refused(b, s(3, 100, 10, vp((1 << 20) + 4), ws), "workspace must be 16-byte")
     _refused(b, s(3, 100, 10, a, ws, vp((1 << 20) + 4)), "packed rows must be 16-byte")
     _refused(b, s(3, 100, 10, a, ws, a, None), "null")
+    _refused(b, L.mvdb_mx4_scan_many_dev(h, a, 3, a, 100, 10, vp((1 << 20) + 2), a, a, a, a, ws, None), "filter is not aligned")
     assert s(0, 100, 10, None, 0, None, None) == 1
     b.close()
 
