@@ -246,9 +246,10 @@ hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int
 			a.out = out + q0 * ldo;
 			const int frags = mx4_product_frags(ksteps);
 			a.groups = (a.nq + 32 * frags - 1) / (32 * frags);
-			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries; but all of a small result's at once
-			const int64_t run = rtiles * a.groups / kMx4ProductGroups;
-			a.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
+			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries (37 x 50 021 x 1000: two steps 9.4 us, one
+			// 11.1 us); but all of a small result's at once
+			const int64_t run = rtiles * a.groups / kMx4ProductGroups, least = rtiles * a.groups >= 512 ? 2 : 1;
+			a.run = (int)(run < least ? least : run > 16 ? 16 : run);
 			const int64_t chunks = (rtiles + a.run - 1) / a.run;
 			const int64_t per_xcd = (chunks + 7) / 8, fit = kMx4BlockBytes / ((int64_t)a.run * 128 * row_bytes);
 			// With up to 16 groups the workgroups in flight spread over enough columns by themselves and share each row at once (1000 x 262 144 x

@@ -65,6 +65,7 @@ class MiniVectorDB:
         self._next_id = 0
         self._vec = np.zeros((0, self.cfg["dim"]), np.float32)      # vecCache / file image
         self._f32_dirty = True
+        self._mx4_dirty = True                                      # the 4-bit store of {"candidates": "mx4"} searches
 
     # ---- open / init / load -------------------------------------------------------
     @classmethod
@@ -96,7 +97,7 @@ class MiniVectorDB:
         if os.path.exists(self.vecPath):
             raw = np.fromfile(self.vecPath, dtype="<f4")
             self._vec = raw[: raw.size // self.cfg["dim"] * self.cfg["dim"]].reshape(-1, self.cfg["dim"]).copy()
-            self._f32_dirty = True
+            self._f32_dirty = self._mx4_dirty = True
         loaded = False
         if os.path.exists(self.dumpPath):
             try:
@@ -166,7 +167,7 @@ class MiniVectorDB:
             grown[: self._vec.shape[0]] = self._vec
             self._vec = grown
         self._vec[ids] = qn
-        self._f32_dirty = True
+        self._f32_dirty = self._mx4_dirty = True
         with open(self.vecPath, "r+b" if os.path.exists(self.vecPath) else "w+b") as f:  # :1038-1070
             for iid, row in zip(ids, qn):
                 f.seek(iid * dim * 4)
@@ -230,8 +231,28 @@ class MiniVectorDB:
                                 resident=self.cfg["preloadVectors"])
             self._f32_dirty = False
 
+    def _query_mx4(self, qs, topK: int, annK: int, allow):
+        """{"candidates": "mx4"} (not in the reference): the candidates are the best of a scan of ALL rows that pass the filter, in
+        microscaled 4 bits (mvdb_mx4_scan_many), instead of a walk through the graph; the rerank is the same.  At most 128
+        candidates, so topK is at most 128; a filter leaves no query short of candidates."""
+        if topK > 128:
+            raise MvdbError(f'candidates "mx4": topK must be at most 128, got {topK}')
+        if not self._vec.shape[0]:
+            nq = len(qs)
+            return np.full((nq, topK), -1, np.int32), np.zeros((nq, topK)), np.zeros(nq, np.int32)
+        if self._mx4_dirty:
+            self.wasm.mx4Attach(self._vec)
+            self._mx4_dirty = False
+        qn, _ = self.wasm.prepareQueries(qs)
+        k = min(128, max(annK, topK))
+        cand, _, count = self.wasm.mx4ScanMany(qn, k, allow)
+        return self.wasm.rerankMany(qn, cand, count, k, topK, allow)
+
     def searchMany(self, queries, opts: Optional[Dict[str, Any]] = None) -> List[List[Dict[str, Any]]]:  # :560-655
         opts = opts or {}
+        candidates = opts.get("candidates") or "graph"            # engine option (not in the reference)
+        if candidates not in ("graph", "mx4"):
+            raise ValueError(f'candidates: "graph" or "mx4", got {candidates!r}')
         if not len(queries):
             return []
         dim = self.cfg["dim"]
@@ -245,7 +266,10 @@ class MiniVectorDB:
             qs[i] = v
         self._sync_f32()
         allow = self._allow_bitmap(opts.get("filter"))
-        ids, l2, n = self.wasm.queryMany(qs, topK, efSearch, annK, allow)
+        if candidates == "mx4":
+            ids, l2, n = self._query_mx4(qs, topK, annK, allow)
+        else:
+            ids, l2, n = self.wasm.queryMany(qs, topK, efSearch, annK, allow)
         out = []
         for qi in range(len(queries)):
             row = []

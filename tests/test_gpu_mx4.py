@@ -533,3 +533,52 @@ def test_host_forms_and_rerank(engines):
     b.mx4Attach(None)
     assert b.mx4Rows() == 0
     b.close()
+
+
+def test_database_candidates(gpu, tmp_path):
+    """MiniVectorDB.searchMany({"candidates": "mx4"}): the four operators' run under the facade, with a filter, deletions, later
+    inserts and a reopened store."""
+    from minivectordb_amd import MiniVectorDB
+    rng = np.random.default_rng(8)
+    n, dim = 3000, 100
+    x = _unit(rng, n + 50, dim)
+    q = _unit(rng, 20, dim)
+    db = MiniVectorDB.open(dict(storageDir=str(tmp_path), dim=dim, capacity=8000, seed=1, preloadVectors=True))
+    assert db.searchMany(q, {"topK": 3, "candidates": "mx4"}) == [[]] * 20
+    db.insertMany([dict(id=f"d{i}", input=x[i], metadata=dict(kind=i % 3)) for i in range(n)])
+
+    def true(rows):  # ids of the nearest among `rows`, and their distances, in 64 bits from the normalised rows
+        xn = x[rows].astype(np.float64) / np.linalg.norm(x[rows].astype(np.float64), axis=1, keepdims=True)
+        qn = q.astype(np.float64) / np.linalg.norm(q.astype(np.float64), axis=1, keepdims=True)
+        d = np.square(qn[:, None] - xn[None]).sum(-1)
+        o = np.argsort(d, 1, kind="stable")
+        return np.asarray(rows)[o], np.take_along_axis(d, o, 1)
+
+    def check(got, rows, topk):
+        ids, d = true(rows)
+        hits = 0
+        for i in range(20):
+            assert len(got[i]) == min(topk, len(rows))
+            by = {f"d{j}": v for j, v in zip(ids[i], d[i])}
+            for r in got[i]:  # what comes back is allowed, in order, and at its f32 distance
+                assert abs(by[r["id"]] - r["score"]) <= 1e-5
+            assert [r["score"] for r in got[i]] == sorted(r["score"] for r in got[i])
+            hits += len({r["id"] for r in got[i]} & {f"d{j}" for j in ids[i][:topk]})
+        assert hits >= 0.95 * 20 * min(topk, len(rows))  # 128 candidates of 4 bits for the best `topk`
+
+    check(db.searchMany(q, {"topK": 10, "candidates": "mx4"}), list(range(n)), 10)
+    check(db.searchMany(q, {"topK": 10, "candidates": "mx4", "filter": {"kind": 1}}), list(range(1, n, 3)), 10)
+    db.removeMany([f"d{i}" for i in range(0, n, 2)])
+    check(db.searchMany(q, {"topK": 5, "candidates": "mx4"}), list(range(1, n, 2)), 5)
+    db.insertMany([dict(id=f"d{i}", input=x[i], metadata=dict(kind=7)) for i in range(n, n + 50)])
+    check(db.searchMany(q, {"topK": 60, "candidates": "mx4", "filter": {"kind": 7}}), list(range(n, n + 50)), 60)
+    assert db.searchMany([x[n + 7]], {"topK": 1, "candidates": "mx4"})[0][0]["id"] == f"d{n + 7}"
+    db.save()
+    db.close()
+    db = MiniVectorDB.open(dict(storageDir=str(tmp_path), dim=dim, capacity=8000, seed=1, preloadVectors=False))
+    check(db.searchMany(q, {"topK": 10, "candidates": "mx4", "filter": {"kind": 7}}), list(range(n, n + 50)), 10)
+    with pytest.raises(Exception, match="at most 128"):
+        db.searchMany(q, {"topK": 129, "candidates": "mx4"})
+    with pytest.raises(ValueError, match="candidates"):
+        db.searchMany(q, {"topK": 1, "candidates": "mx5"})
+    db.close()
