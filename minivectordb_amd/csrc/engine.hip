@@ -421,7 +421,7 @@ int DeviceIndex::patch(const HostGraph &g, std::string &err)
 // mvdb_search_many_dev_noalloc keeps its visited bitmaps here instead of in hipMalloc'ed memory.
 // `scratch` is a host-side stand-in, not a device address: host code only ever uses the per-device
 // pointer hipGetSymbolAddress returned (resolve_scratch, with that device current), as the kernel
-// argument and for hipMemsetAsync.  Every GPU the library runs on holds its own 64 MiB copy.
+// argument.  Every GPU the library runs on holds its own 64 MiB copy.
 constexpr size_t kNoAllocScratchBytes = (size_t)64 << 20;
 constexpr int kMaxDevices = 16;
 static __device__ __align__(256) unsigned char scratch[kNoAllocScratchBytes];
@@ -1208,6 +1208,15 @@ __global__ __launch_bounds__(256) void zero_nt_kernel(uint4 *p, size_t n16)
 		__builtin_nontemporal_store(z, reinterpret_cast<v4u_t *>(p) + i);
 }
 
+__global__ __launch_bounds__(256) void zero_words_kernel(int32_t *p, size_t n)
+{
+	for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) p[i] = 0;
+}
+void zero_words(int32_t *p, size_t n, hipStream_t s)
+{
+	hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1024)), dim3(256), 0, s, p, n);
+}
+
 // shared by mvdb_search_many_dev (sorted lists, the bridge contract) and the fused query path
 // (set_only: see TraverseArgs)
 int search_many_dev_impl(mvdb_index *h, const int8_t *d_q, int nq, int k, int32_t *d_out_ids, float *d_out_dist,
@@ -1358,8 +1367,9 @@ int mvdb_search_many_dev_noalloc(mvdb_index *h, const int8_t *d_q, int nq, int k
 	hipStream_t s = static_cast<hipStream_t>(stream);
 	const HostGraph &g = h->g;
 	if (g.entry_point == -1 || g.max_elements <= 0 || k <= 0 || !g.present(g.entry_point)) {  // hnsw.ts:961-967
-		HIP_OK(h, hipMemsetAsync(d_out_count, 0, (size_t)nq * 4, s));
-		if (d_ctr) HIP_OK(h, hipMemsetAsync(d_ctr, 0, (size_t)nq * sizeof(mvdb_query_counters), s));
+		zero_words(d_out_count, (size_t)nq, s);
+		if (d_ctr) zero_words(reinterpret_cast<int32_t *>(d_ctr), (size_t)nq * (sizeof(mvdb_query_counters) / 4), s);
+		HIP_OK(h, hipGetLastError());
 		return 1;
 	}
 	TraverseArgs a;
@@ -1371,7 +1381,11 @@ int mvdb_search_many_dev_noalloc(mvdb_index *h, const int8_t *d_q, int nq, int k
 		return 0;
 	}
 	void *vis = g_scratch_ptr[d];                // never the array's name: that is not a device address
-	HIP_OK(h, hipMemsetAsync(vis, 0, need, s));  // the array keeps the last call's bits: cleared every call
+	// the array keeps the last call's bits: cleared every call, by a kernel (a memset node of a captured graph has given wrong results on replays
+	// after the first)
+	const size_t n16 = need / 16;  // (rows are padded to 256 bytes)
+	hipLaunchKernelGGL(zero_nt_kernel, dim3((unsigned)std::min<size_t>((n16 + 255) / 256, 2048)), dim3(256), 0, s, static_cast<uint4 *>(vis), n16);
+	HIP_OK(h, hipGetLastError());
 	a.q = d_q;
 	a.nq = nq;
 	a.visited = vis;
