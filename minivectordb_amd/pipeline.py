@@ -230,6 +230,8 @@ class ResidentMx4:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._index = self.device.index
         self._raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the objects around it
+        self._u8, self._i32, self._f32 = (torch.empty(1, dtype=t, device=self.device).new_empty if torch.cuda.is_available() else None
+                                          for t in (torch.uint8, torch.int32, torch.float32))  # new tensors of a type here
         self._cfg = None
 
     def _engine(self):
@@ -278,7 +280,7 @@ class ResidentMx4:
             ld = dim
         if inner != 1 or ld < dim:
             raise MvdbError(f"mx4 quantize: components have to follow each other and rows not overlap, got strides {x.stride()}")
-        out = torch.empty((rows, self._row_bytes), dtype=torch.uint8, device=self.device)
+        out = self._u8((rows, self._row_bytes))
         if not self.L.mvdb_mx4_quantize_dev(h, x.data_ptr(), dtype, rows, ld, out.data_ptr(), self._raw_stream(self._index)):
             self.b._check(0)
         return out
@@ -287,7 +289,7 @@ class ResidentMx4:
         """Packed rows -> the values they stand for, f32 [rows, dim]."""
         h = self._engine()
         rows = self._packed(packed, "mx4 expand")
-        out = torch.empty((rows, self._dim), dtype=torch.float32, device=self.device)
+        out = self._f32((rows, self._dim))
         if not self.L.mvdb_mx4_expand_dev(h, packed.data_ptr(), rows, out.data_ptr(), self._raw_stream(self._index)):
             self.b._check(0)
         return out
@@ -297,7 +299,7 @@ class ResidentMx4:
         h = self._engine()
         nq, n = self._packed(q, "mx4 product (queries)"), self._packed(rows, "mx4 product (rows)")
         if out is None:
-            out = torch.empty((nq, n), dtype=torch.float32, device=self.device)
+            out = self._f32((nq, n))
             ldo = n
         else:
             self._on_device(out, "mx4 product (out)")
@@ -322,12 +324,9 @@ class ResidentMx4:
             bits = allow.data_ptr()
         if not 1 <= k <= 128:
             raise MvdbError(f"mx4 scan: k must be 1..128, got {k}")
-        dev = self.device
-        ids = torch.empty((nq, k), dtype=torch.int32, device=dev)
-        val = torch.empty((nq, k), dtype=torch.float32, device=dev)
-        cnt = torch.empty((nq,), dtype=torch.int32, device=dev)
+        ids, val, cnt = self._i32((nq, k)), self._f32((nq, k)), self._i32(nq)
         need = self.L.mvdb_mx4_scan_workspace(h, nq, n, k)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        ws = self._u8(need)
         if not self.L.mvdb_mx4_scan_many_dev(h, q.data_ptr(), nq, rows.data_ptr(), n, k, bits, ids.data_ptr(), val.data_ptr(), cnt.data_ptr(),
                                              ws.data_ptr(), need, self._raw_stream(self._index)):
             self.b._check(0)
