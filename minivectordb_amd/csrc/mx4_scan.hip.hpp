@@ -5,12 +5,12 @@
 // and rows whose product is NaN are no candidates; a row is taken out by giving its blocks the scale 255, which makes every product NaN,
 // and a NaN is never >= a bound.
 //
-// Two ways, by the number of queries:
+// Two ways, by the number of queries (1 M rows x 384, k 10: 8 queries 56 us in chunks, 9 queries 75 us in levels, 64 queries 79 us):
 //
-// CHUNKS (few queries): a workgroup computes the products of its own run of rows, keeps them in LDS and picks the best k of each
+// CHUNKS (up to 8 queries): a workgroup computes the products of its own run of rows, keeps them in LDS and picks the best k of each
 // query there; a second launch picks the best k of those.  Every row is read once, and two launches are all there is.
 //
-// LEVELS (many queries): the rows are taken in levels of 64-row tiles, each about `ratio` times the one before it: level 0 is every
+// LEVELS (more): the rows are taken in levels of 64-row tiles, each about `ratio` times the one before it: level 0 is every
 // ratio^L-th tile, level l the tiles that are multiples of ratio^(L - l) and not of ratio^(L - l + 1).  After a level the k-th best key so
 // far is a bound: k rows are at least that good, so only keys above it matter, and as the rows seen so far are spread evenly over the
 // store about k (ratio - 1) keys of the next level are (whatever order the rows are in, unless they repeat with the tiles' period).
@@ -371,12 +371,12 @@ __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS>
 #pragma unroll
 	for (int s = 0; s < KS; s++) {
 #pragma unroll
-			for (int c = 0; c < C; c++) {
-				const mx4_v16f &in = s == 0 ? zero : acc[c];
-				acc[c] = (s & 1) ? mx4_mfma<2, 2>(a.d[s], a.sc[s / 2], b[c].d[s], b[c].sc[s / 2], in)
-				                 : mx4_mfma<0, 0>(a.d[s], a.sc[s / 2], b[c].d[s], b[c].sc[s / 2], in);
-			}
+		for (int c = 0; c < C; c++) {
+			const mx4_v16f &in = s == 0 ? zero : acc[c];
+			acc[c] = (s & 1) ? mx4_mfma<2, 2>(a.d[s], a.sc[s / 2], b[c].d[s], b[c].sc[s / 2], in)
+			                 : mx4_mfma<0, 0>(a.d[s], a.sc[s / 2], b[c].d[s], b[c].sc[s / 2], in);
 		}
+	}
 	// A matrix instruction reads its operands from all lanes, whatever the execution mask.  The compiler may move it into a branch that only
 	// some lanes take when nothing but that branch uses the result, and the shifts of the scales with it, which do obey the mask: this use
 	// keeps both here.
@@ -387,8 +387,8 @@ __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS>
 // ---------------------------------------------------------------------------------------------- chunks
 constexpr int kMx4ChunkQ = 8;        // queries of a workgroup
 constexpr int kMx4ChunkRows = 2048;  // rows a workgroup, at most
-
 constexpr int kMx4ChunkThreads = 512;
+constexpr int64_t kMx4ChunkKeys = 1 << 17;  // keys that the chunks leave for a query, at most: one workgroup goes through them
 static_assert(kMx4ChunkThreads / 64 >= kMx4ChunkQ, "a wave for each query");
 
 // A wave takes 32 rows at a time, the next ones on their way meanwhile.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
@@ -489,7 +489,7 @@ struct Mx4Level {
 	const uint8_t *q, *rows;
 	const uint32_t *allow;
 	int nq, n;
-	int64_t step;     // see mx4_level_tile
+	int64_t step;     // see mx4_tile_row
 	uint64_t skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
 	int tiles;
 	const mx4_key *bound;  // [nq], 0 = none
@@ -766,7 +766,6 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		__builtin_amdgcn_s_barrier();                     // ... and everybody's, and the group before it is done with
 		asm volatile("" ::: "memory");
 		if (AHEAD) mx4_load_frag<KS>(f0, image(t, 0), half);
-#pragma unroll 2
 		for (int u = t; u < t + G && u < ntiles; u++) {
 			if (u + G < ntiles) fetch(u + G);
 			const int64_t row0 = mx4_tile_row(a, split + u * splits);
@@ -867,12 +866,12 @@ inline size_t mx4_up(size_t b) { return (b + 255) & ~(size_t)255; }
 inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 {
 	Mx4Plan p{};
-	p.chunks = nq <= kMx4ChunkQ;
+	// about two workgroups a compute unit
+	const int64_t c = (((int64_t)n + 511) / 512 + 127) / 128 * 128;
+	p.chunk = (int)(c < 512 ? 512 : c > kMx4ChunkRows ? kMx4ChunkRows : c);
+	p.parts = (int)(((int64_t)n + p.chunk - 1) / p.chunk);
+	p.chunks = nq <= kMx4ChunkQ && (int64_t)p.parts * k <= kMx4ChunkKeys;
 	if (p.chunks) {
-		int64_t c = ((int64_t)n + 511) / 512;  // about two workgroups a compute unit
-		c = (c + 127) / 128 * 128;
-		p.chunk = (int)(c < 512 ? 512 : c > kMx4ChunkRows ? kMx4ChunkRows : c);
-		p.parts = (int)(((int64_t)n + p.chunk - 1) / p.chunk);
 		p.ws = mx4_up((size_t)nq * p.parts * k * 8 + 8);
 		return p;
 	}
@@ -953,7 +952,6 @@ template <int KS>
 hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uint8_t *rows, int n, int k, const uint32_t *allow,
                            const Mx4Out &last, void *ws, hipStream_t s)
 {
-	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	uint8_t *w = static_cast<uint8_t *>(ws);
 	auto take = [&](size_t bytes) -> void * {
 		void *at = w;
