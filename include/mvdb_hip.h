@@ -75,6 +75,8 @@ void mvdb_destroy(mvdb_index *h);
 const char *mvdb_last_error(const mvdb_index *h);
 /* 1 when a HIP device whose gcnArchName starts with "gfx950" is visible to this process */
 int mvdb_device_available(void);
+/* the HIP device ordinal that the handle works on (-1 at creation is resolved there) */
+int mvdb_device(const mvdb_index *h);
 
 /* ---- index state (WasmBridge getters/setters) ---------------------------- */
 int mvdb_get_max_ef(void);                        /* get_max_ef, hnsw.ts:90       */

@@ -71,6 +71,7 @@ SYMBOLS = [
     ("mvdb_dist_many", _i, [_vp, _vp, _i, _vp, _i, _i, _vp]),
     ("mvdb_scan_many", _i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
     ("mvdb_scan_many_dev", _i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    ("mvdb_device", _i, [_vp]),
     ("mvdb_mx4_row_bytes", _i, [_vp]),
     ("mvdb_mx4_quantize_dev", _i, [_vp, _vp, _i, _i64, _i64, _vp, _vp]),
     ("mvdb_mx4_expand_dev", _i, [_vp, _vp, _i64, _vp, _vp]),

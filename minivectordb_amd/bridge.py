@@ -417,6 +417,8 @@ class HipBridge:
         ids are a candidate list for rerankMany."""
         q = self._rows(q_f32, np.float32, "mx4ScanMany")
         nq = q.shape[0]
+        if not 1 <= int(k) <= 128:
+            raise MvdbError(f"mx4ScanMany: k must be 1..128, got {k}")
         with self._lock:
             allow = None
             if allow_bitmap is not None:
@@ -424,8 +426,8 @@ class HipBridge:
                 need = (self.mx4Rows() + 31) // 32
                 if allow.size < need:
                     raise MvdbError(f"allow bitmap too short: {allow.size} words for {self.mx4Rows()} rows ({need} needed)")
-            ids = np.full((nq, max(int(k), 1)), -1, np.int32)
-            val = np.zeros((nq, max(int(k), 1)), np.float32)
+            ids = np.full((nq, int(k)), -1, np.int32)
+            val = np.zeros((nq, int(k)), np.float32)
             cnt = np.zeros(nq, np.int32)
             self._check(self._L.mvdb_mx4_scan_many(self.handle, _ptr(q), nq, int(k), _ptr(allow), _ptr(ids), _ptr(val), _ptr(cnt)))
         return ids, val, cnt

@@ -1871,12 +1871,19 @@ struct MaybeTimer {
 	MaybeTimer(mvdb_index *h, int stage, hipStream_t s)
 	{
 		hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
-		if (!h->timing || hipStreamIsCapturing(s, &c) != hipSuccess || c != hipStreamCaptureStatusNone) return;
+		if (!h->timing) return;
+		if (hipStreamIsCapturing(s, &c) != hipSuccess) {
+			(void)hipGetLastError();  // (asked, not failed: the launches report their own)
+			return;
+		}
+		if (c != hipStreamCaptureStatusNone) return;
 		t.reset(new StageTimer(h, stage, s));
 	}
 };
 
 }  // namespace
+
+int mvdb_device(const mvdb_index *h) { return h->device; }
 
 int mvdb_mx4_row_bytes(const mvdb_index *h) { return mx4_row_bytes(h->cfg.dim); }
 

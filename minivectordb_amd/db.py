@@ -85,6 +85,7 @@ class MiniVectorDB:
                             capacity=c["capacity"], seed=c["seed"], resultsCap=c["resultsCap"]))
         self.wasmMaxEf = self.wasm.getMaxEf()
         self.capacity = c["capacity"]
+        self._f32_dirty = self._mx4_dirty = True                  # a new engine holds neither store
         self.isReady = True
 
     def load(self):                                               # :710-749

@@ -222,22 +222,25 @@ class ResidentMx4:
 
     def __init__(self, bridge: HipBridge, device: torch.device):
         self.b, self.L = bridge, bridge._L
-        bridge.handle  # an initialised bridge is needed
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise MvdbError(f"ResidentMx4: a GPU device is needed, got {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._index = self.device.index
+        self._cfg = None
+        self._engine()
         self._raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the objects around it
         self._u8, self._i32, self._f32 = (torch.empty(1, dtype=t, device=self.device).new_empty if torch.cuda.is_available() else None
                                           for t in (torch.uint8, torch.int32, torch.float32))  # new tensors of a type here
-        self._cfg = None
 
     def _engine(self):
         """The bridge's handle; dim and row_bytes follow it when the bridge is initialised again."""
         b = self.b
         if b._cfg is not self._cfg or not b._h:
+            at = self.L.mvdb_device(b.handle)
+            if at != self._index:
+                raise MvdbError(f"ResidentMx4: the bridge works on cuda:{at}, not on {self.device}")
             self._dim, self._row_bytes, self._cfg = b._dim(), b.mx4RowBytes(), b._cfg
         return b._h
 

@@ -385,6 +385,10 @@ def test_far_offsets(engines):
     assert torch.equal(ids[:, 0].long(), torch.arange(n - 70, n - 65, device="cuda"))
     ids, val, cnt = mx.scan_many(q, rows, 3)
     assert torch.equal(ids[:, 0].long(), torch.arange(n - 70, n, device="cuda"))
+    ids, val, cnt = mx.scan_many(q[:3], rows, 128)  # more keys than chunks may leave
+    s3 = mx.product(q[:3], rows)
+    assert torch.equal(val, s3.topk(128, dim=1).values) and torch.equal(s3.gather(1, ids.long()), val)
+    del s3
     v = mx.expand(rows[-3000:])
     assert torch.equal(mx.quantize(v)[:, :512], mx.quantize(v.double().float())[:, :512])
     out = mx.product(rows[-300:], rows)  # 2.46e9 products
@@ -581,4 +585,7 @@ def test_database_candidates(gpu, tmp_path):
         db.searchMany(q, {"topK": 129, "candidates": "mx4"})
     with pytest.raises(ValueError, match="candidates"):
         db.searchMany(q, {"topK": 1, "candidates": "mx5"})
+    db.close()
+    db.init()  # the same object on a new engine, which holds neither store of rows
+    check(db.searchMany(q, {"topK": 10, "candidates": "mx4", "filter": {"kind": 7}}), list(range(n, n + 50)), 10)
     db.close()

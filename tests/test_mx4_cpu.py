@@ -124,6 +124,9 @@ def test_host_entry_points_refuse():
     assert b.mx4Rows() == 0
     with pytest.raises(MvdbError, match="no 4-bit store"):
         b.mx4ScanMany(x, 5)
+    for k in (0, 129, 1 << 40):  # refused before anything of that size is made
+        with pytest.raises(MvdbError, match="k must be 1..128"):
+            b.mx4ScanMany(x, k)
     with pytest.raises(MvdbError, match="no 4-bit store"):
         b.mx4ProductMany(x)
     with pytest.raises(MvdbError, match="dim"):
@@ -142,6 +145,8 @@ def test_resident_refuses():
     b = _bridge(64)
     with pytest.raises(MvdbError, match="GPU device"):
         ResidentMx4(b, torch.device("cpu"))
+    with pytest.raises(MvdbError, match="works on cuda:0"):
+        ResidentMx4(b, torch.device("cuda", 1))
     mx = ResidentMx4(b, torch.device("cuda", 0))
     with pytest.raises(MvdbError, match="cuda:0"):
         mx.quantize(torch.zeros((2, 64)))
