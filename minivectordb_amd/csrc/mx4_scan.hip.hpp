@@ -14,8 +14,8 @@
 // ratio^L-th tile, level l the tiles that are multiples of ratio^(L - l) and not of ratio^(L - l + 1).  After a level the k-th best key so
 // far is a bound: k rows are at least that good, so only keys above it matter, and as the rows seen so far are spread evenly over the
 // store about k (ratio - 1) keys of the next level are (whatever order the rows are in, unless they repeat with the tiles' period).
-// Level 0 has no bound: it is one chunk.  From then on a lane whose product passes the bound appends the key to a list of its
-// own, which needs no atomics: a lane only ever sees one query a fragment, and the tiles are dealt out in turn, so lists stay short.
+// Level 0 has no bound: it is one chunk.  From then on a lane whose product passes the bound appends it to a list of its own,
+// which needs no atomics: a lane only ever sees one query a fragment, and the tiles are dealt out in turn, so lists stay short.
 // mx4_pick_kernel gathers a query's lists after every level and keeps the best k.  A list that overflows marks its query, and
 // mx4_rescue_kernel does those over, one workgroup each.
 #pragma once
@@ -304,15 +304,27 @@ __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *ke
 }
 
 // T threads per query (a workgroup, or a wave of one): the best k of what it had and of its lists, CAP keys in all
-constexpr int kMx4List = 64;       // keys of a list
+// What a list holds: keys, or (many queries) records of four neighbouring rows of which at least one may be a candidate: the first one's id, and the
+// products (NaN: a row that does not count).
+struct __attribute__((packed, aligned(4))) Mx4Record {
+	float v[4];
+	unsigned id;
+};
+__device__ __forceinline__ void mx4_keys_of(const mx4_key &r, mx4_key (&key)[1]) { key[0] = r; }
+__device__ __forceinline__ void mx4_keys_of(const Mx4Record &r, mx4_key (&key)[4])
+{
+#pragma unroll
+	for (int t = 0; t < 4; t++) key[t] = mx4_make_key(r.v[t], r.id + t);
+}
+
 // Keys of all lists of a query.  The plan sees to it that a random order of the rows stays far below them; what asks for more is a run of neighbouring
 // rows that are all candidates and that the levels before have missed, at most 64 x ratio of them.
 constexpr int kMx4Gather = 2048, kMx4GatherFewQueries = 4096;
 constexpr int kMx4GatherWave = 768;  // the most that a wave deals with
 
-template <int T, int CAP>
-__global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, const int32_t *counts, int parts, const mx4_key *before, const int32_t *nbefore,
-                                                       int nq, int k, Mx4Out o, int32_t *over)
+template <int T, int CAP, typename R, int LISTS, int P>
+__global__ __launch_bounds__(256) void mx4_pick_kernel(const R *lists, const int32_t *counts, int parts, int list, const mx4_key *before,
+                                                       const int32_t *nbefore, const mx4_key *bound, int nq, int k, Mx4Out o, int32_t *over)
 {
 	__shared__ Mx4PickLds ls[256 / T];
 	__shared__ __attribute__((aligned(16))) mx4_key keyss[256 / T][CAP];
@@ -327,6 +339,7 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 #pragma unroll
 	for (int j = 0; j < (kMx4ScanMaxK + T - 1) / T; j++) old[j] = j * T + tid < kMx4ScanMaxK ? before[q * kMx4ScanMaxK + j * T + tid] : 0;
 	const int had = nbefore[q];
+	const mx4_key beat = bound[q];  // (this kernel writes it, after the last of its threads has read it)
 	if (tid == 0) {
 		total = had;
 		lost = 0;
@@ -335,21 +348,52 @@ __global__ __launch_bounds__(256) void mx4_pick_kernel(const mx4_key *lists, con
 #pragma unroll
 	for (int j = 0; j < (kMx4ScanMaxK + T - 1) / T; j++)
 		if (j * T + tid < had) keys[j * T + tid] = old[j];
-#pragma unroll 4
-	for (int i = tid; i < parts; i += T) {
-		const mx4_key *src = lists + (q * parts + i) * kMx4List;
-		const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(src);  // most lists hold none, one or two
-		int c = counts[q * parts + i];
-		if (c > 0) {
-			if (c > kMx4List) {
-				lost = 1;
-				c = kMx4List;
+	// LISTS lists a thread at a time, and P records of each: loads that wait for nothing, as many as most lists hold
+	constexpr int N = sizeof(R) == sizeof(mx4_key) ? 1 : 4;
+	auto gather = [&](const R (&r)[P], int count) {
+		mx4_key key[P][N];
+		int n = 0;
+#pragma unroll
+		for (int j = 0; j < P; j++) {
+			mx4_keys_of(r[j], key[j]);
+#pragma unroll
+			for (int t = 0; t < N; t++) {
+				key[j][t] = j < count && (N == 1 || key[j][t] > beat) ? key[j][t] : 0;  // (a key that stands alone has been compared)
+				n += key[j][t] ? 1 : 0;
 			}
-			const int at = atomicAdd(&total, c);
-			if (at < CAP) keys[at] = two.x;
-			if (c > 1 && at + 1 < CAP) keys[at + 1] = two.y;
-			for (int j = 2; j < c; j++)
-				if (at + j < CAP) keys[at + j] = src[j];
+		}
+		int at = atomicAdd(&total, n);
+#pragma unroll
+		for (int j = 0; j < P; j++)
+#pragma unroll
+			for (int t = 0; t < N; t++)
+				if (key[j][t]) {
+					if (at < CAP) keys[at] = key[j][t];
+					at++;
+				}
+	};
+	for (int i = tid; i < parts; i += LISTS * T) {
+		const R *src[LISTS];
+		R r[LISTS][P];
+		int c[LISTS];
+#pragma unroll
+		for (int u = 0; u < LISTS; u++) {
+			const int at = i + u * T < parts ? i + u * T : parts - 1;
+			src[u] = lists + (q * parts + at) * list;
+			c[u] = counts[q * parts + at];
+#pragma unroll
+			for (int j = 0; j < P; j++) r[u][j] = src[u][j];  // (a list has 32 places at least)
+		}
+#pragma unroll
+		for (int u = 0; u < LISTS; u++) {
+			if (i + u * T >= parts || c[u] == 0) continue;
+			if (c[u] == list - 1) lost = 1;
+			gather(r[u], c[u]);
+			for (int at = P; at < c[u]; at += P) {
+#pragma unroll
+				for (int j = 0; j < P; j++) r[u][j] = src[u][at + j < c[u] ? at + j : at];
+				gather(r[u], c[u] - at);
+			}
 		}
 	}
 	mx4_sync<T>();
@@ -493,9 +537,9 @@ struct Mx4Level {
 	uint64_t skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
 	int tiles;
 	const mx4_key *bound;  // [nq], 0 = none
-	mx4_key *lists;   // [nq][parts][kMx4List]
-	int32_t *counts;  // [nq][parts] keys of a list (may run past kMx4List)
-	int parts;
+	void *lists;       // [nq][parts][list] keys or records
+	int32_t *counts;   // [nq][parts] how many a list holds; list - 1: some may be lost
+	int parts, list;
 };
 
 // tile i of a level, first row: i / (ratio - 1) by a multiplication, exact for i (ratio - 1) < 2^32 (i < 2^25)
@@ -518,11 +562,10 @@ struct Mx4Queries {
 	Mx4Frag<KS> b[C];
 	float bound[C];
 	mx4_key bkey[C];
-	unsigned list[C];  // byte offset of the list's first key (262 144 lists at most: mx4_plan)
-	int count[C];
+	unsigned at[C], last[C];  // byte offsets of the list's next place and of its last
 };
 
-template <int KS, int C>
+template <typename R, int KS, int C>
 __device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS, C> &w, const Mx4Level &a, int q0, int part, int half, int r32)
 {
 #pragma unroll
@@ -533,16 +576,16 @@ __device__ __forceinline__ void mx4_load_queries(Mx4Queries<KS, C> &w, const Mx4
 		w.bkey[c] = a.bound[qs];
 		// no query in this column: nothing is >= NaN
 		w.bound[c] = q >= a.nq ? __uint_as_float(0x7fc00000u) : w.bkey[c] ? mx4_key_value(w.bkey[c]) : -__builtin_inff();
-		w.list[c] = ((unsigned)qs * a.parts + part) * (kMx4List * 8);
-		w.count[c] = 0;
+		w.at[c] = ((unsigned)qs * a.parts + part) * a.list * (unsigned)sizeof(R);
+		w.last[c] = w.at[c] + (a.list - 1) * (unsigned)sizeof(R);
 	}
 }
-template <int KS, int C>
+template <typename R, int KS, int C>
 __device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS, C> &w, const Mx4Level &a, int q0, int part, int r32)
 {
 #pragma unroll
 	for (int c = 0; c < C; c++)
-		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = w.count[c];
+		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = a.list - 1 - (int)((w.last[c] - w.at[c]) / sizeof(R));
 }
 
 // Test of a lane's 16 products with each of its queries: the largest of every four, and whether any may be a candidate.
@@ -560,11 +603,21 @@ __device__ __forceinline__ bool mx4_test(const Mx4Queries<KS, C> &w, const mx4_v
 	return any;
 }
 
-// Append what passed; rows row0 .. + 31.
-template <int KS, int C>
+// One more in this lane's list.  The last place of a list is written over and over, and its number says that some may be lost.
+template <typename R, int KS, int C>
+__device__ __forceinline__ void mx4_append_one(Mx4Queries<KS, C> &w, const Mx4Level &a, int c, const R &r)
+{
+	*reinterpret_cast<R *>(static_cast<char *>(a.lists) + w.at[c]) = r;
+	const unsigned next = w.at[c] + (unsigned)sizeof(R);
+	w.at[c] = next < w.last[c] ? next : w.last[c];
+}
+
+// Append what passed; rows row0 .. + 31.  As keys, one by one; or four products at a time, in one record, where which of them pass is found by
+// mx4_pick_kernel.  Records take fewer instructions here, where they keep the matrix instructions waiting, and more there (1 M rows x 384, k 100:
+// 1000 queries 316 us with keys, 288 with records); with few queries a wave has few candidates and mx4_pick_kernel many lists (64 queries: 104 and 127).
+template <typename R, int KS, int C>
 __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], const float (&m)[C][4], int64_t row0, int half)
 {
-	char *lists = reinterpret_cast<char *>(a.lists);
 	unsigned id0 = (unsigned)row0 + 4 * half;
 	asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
 #pragma unroll
@@ -572,17 +625,19 @@ __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level 
 #pragma unroll
 		for (int g = 0; g < 4; g++)
 			if (__ballot(m[c][g] >= w.bound[c])) {
+				if constexpr (sizeof(R) == sizeof(Mx4Record)) {
+					// (an equal product behind the bound's id is no candidate: rows that are all alike fill no lists)
+					const unsigned id = id0 + 8 * g;
+					if ((m[c][g] > w.bound[c]) | ((m[c][g] >= w.bound[c]) & (~id > (unsigned)w.bkey[c])))
+						mx4_append_one(w, a, c, Mx4Record{{acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]}, id});
+				} else {
 #pragma unroll
-				for (int j = 0; j < 4; j++) {
-					const float v = acc[c][4 * g + j];
-					if (__ballot(v >= w.bound[c])) {
-						const unsigned b = __float_as_uint(v + 0.f);  // mx4_make_key of a number
-						const mx4_key key = ((mx4_key)(b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) << 32) | ~(id0 + 8 * g + j);
-						if (v >= w.bound[c] && key > w.bkey[c]) {
-							// (a list that is full loses its last key, and says so by its count)
-							const unsigned at = w.list[c] + 8u * (unsigned)(w.count[c] < kMx4List ? w.count[c] : kMx4List - 1);
-							*reinterpret_cast<mx4_key *>(lists + at) = key;
-							w.count[c]++;
+					for (int j = 0; j < 4; j++) {
+						const float v = acc[c][4 * g + j];
+						if (__ballot(v >= w.bound[c])) {
+							const unsigned b = __float_as_uint(v + 0.f);  // mx4_make_key of a number
+							const mx4_key key = ((mx4_key)(b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) << 32) | ~(id0 + 8 * g + j);
+							if (v >= w.bound[c] && key > w.bkey[c]) mx4_append_one(w, a, c, key);
 						}
 					}
 				}
@@ -603,7 +658,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	constexpr int C = mx4_stream_frags(KS);
 	Mx4Queries<KS, C> w;
-	mx4_load_queries(w, a, group * 32 * C, 2 * first + half, half, r32);
+	mx4_load_queries<mx4_key>(w, a, group * 32 * C, 2 * first + half, half, r32);
 	const unsigned total = 2 * (unsigned)a.tiles;
 	// half tile i: its first row and which of its rows count, and (unless none does) the rows
 	auto load = [&](unsigned i, Mx4Frag<KS> &f, int64_t &row0, unsigned &keep) {
@@ -625,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 		mx4_v16f acc[C];
 		mx4_tile<KS, C>(f, w.b, acc);
 		float m[C][4];
-		if (__builtin_expect(__ballot(mx4_test(w, acc, m)) != 0, 0)) mx4_append(w, a, acc, m, row0, half);
+		if (__builtin_expect(__ballot(mx4_test(w, acc, m)) != 0, 0)) mx4_append<mx4_key>(w, a, acc, m, row0, half);
 	};
 	if constexpr (KS <= 12) {
 		Mx4Frag<KS> f0, f1;
@@ -655,7 +710,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 			use(f, row0, keep);
 		}
 	}
-	mx4_store_counts(w, a, group * 32 * C, 2 * first + half, r32);
+	mx4_store_counts<mx4_key>(w, a, group * 32 * C, 2 * first + half, r32);
 }
 
 // Tiles of 64 rows, staged in LDS for up to 8 waves of 64 queries each.  Groups of tiles come by LDS-DMA into two places in turn: while one group is
@@ -686,7 +741,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	constexpr int G = mx4_stage_group(KS);
 	const int q0 = (qtile * nwaves + wave) * 64;
 	Mx4Queries<KS, 2> w;
-	mx4_load_queries(w, a, q0, 2 * split + half, half, r32);
+	mx4_load_queries<Mx4Record>(w, a, q0, 2 * split + half, half, r32);
 	const int ntiles = split < a.tiles ? (a.tiles - split + splits - 1) / splits : 0;
 
 	using lds_ptr_t = __attribute__((address_space(3))) void *;
@@ -733,7 +788,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		if constexpr (!PIPED) {
 			mx4_tile<KS, 2>(f, w.b, now);
 			float m[2][4];
-			if (__builtin_expect(__ballot(mx4_test(w, now, m)) != 0, 0)) mx4_append(w, a, now, m, row, half);
+			if (__builtin_expect(__ballot(mx4_test(w, now, m)) != 0, 0)) mx4_append<Mx4Record>(w, a, now, m, row, half);
 			return;
 		}
 		const mx4_v16f zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -759,7 +814,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		bool any = false;
 #pragma unroll
 		for (int c = 0; c < 2; c++) any |= __builtin_fmaxf(__builtin_fmaxf(m[c][0], m[c][1]), __builtin_fmaxf(m[c][2], m[c][3])) >= w.bound[c];
-		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append(w, a, then, m, row, half);
+		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append<Mx4Record>(w, a, then, m, row, half);
 	};
 	for (int t = 0; t < ntiles; t += G) {
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the group is there ...
@@ -787,9 +842,9 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	}
 	if (PIPED) {
 		float m[2][4];
-		if (__ballot(mx4_test(w, accB, m))) mx4_append(w, a, accB, m, rowB, half);
+		if (__ballot(mx4_test(w, accB, m))) mx4_append<Mx4Record>(w, a, accB, m, rowB, half);
 	}
-	mx4_store_counts(w, a, q0, 2 * split + half, r32);
+	mx4_store_counts<Mx4Record>(w, a, q0, 2 * split + half, r32);
 }
 
 // The queries that lost keys, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
@@ -854,10 +909,10 @@ constexpr int kMx4MostRatio = 10, kMx4MostRatioFew = 52;  // many queries: 4 to 
 
 struct Mx4Plan {
 	bool chunks, few;  // few: keys that a query gathers in a level
-	int chunk, parts;  // chunks: rows of one, how many; levels: lists of a query
+	int chunk, parts, list;  // chunks: rows of one, how many; levels: lists of a query, places of a list
 	int levels, ratio, first_rows;  // levels after level 0; rows of level 0 (a multiple of 64)
 	int64_t step0;
-	int slab, qgroups, qtiles, splits;
+	int slab, qgroups, qtiles, splits, record;  // record: bytes of what a list holds
 	size_t ws;
 };
 
@@ -909,8 +964,14 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 1) : most_waves);
 	}
 	p.parts = 2 * p.splits;
+	// a list's share of a level's candidates, with the same margin, and room for neighbouring rows that are all candidates, three tiles of them in
+	// records and two in keys; whole cache lines, so that the first few lie in one
+	const double share = (double)k * (p.ratio > 1 ? p.ratio - 1 : 0) / p.parts;
+	const int least = (int)(share + 6 * std::sqrt(share)) + (many ? 25 : 60), line = many ? 32 : 16;
+	p.list = (least + line - 1) / line * line;
+	p.record = many ? sizeof(Mx4Record) : sizeof(mx4_key);
 	p.ws = mx4_up((size_t)p.slab * kMx4ScanMaxK * 8) + mx4_up((size_t)p.slab * 8) + 2 * mx4_up((size_t)p.slab * 4);
-	if (p.levels) p.ws += mx4_up((size_t)p.slab * p.parts * 4) + mx4_up((size_t)p.slab * p.parts * kMx4List * 8);
+	if (p.levels) p.ws += mx4_up((size_t)p.slab * p.parts * 4) + mx4_up((size_t)p.slab * p.parts * p.list * p.record);
 	return p;
 }
 
@@ -972,7 +1033,8 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	a.parts = p.parts;
 	if (p.levels) {
 		a.counts = static_cast<int32_t *>(take((size_t)p.slab * p.parts * 4));
-		a.lists = static_cast<mx4_key *>(take((size_t)p.slab * p.parts * kMx4List * 8));
+		a.list = p.list;
+		a.lists = take((size_t)p.slab * p.parts * p.list * p.record);
 	}
 	const Mx4Out mid = {nullptr, nullptr, nullptr, best, bound, nbest};
 	const bool stage = p.qtiles > 0;
@@ -1002,13 +1064,13 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 		else
 			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
 		if (p.few)
-			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherWave>), dim3((nq + 3) / 4), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherWave, Mx4Record, 1, 4>), dim3((nq + 3) / 4), dim3(256), 0, s, static_cast<const Mx4Record *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
 			                   l < p.levels ? mid : last, over);
 		else if (!stage)
-			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4GatherFewQueries>), dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4GatherFewQueries, mx4_key, 4, 2>), dim3(nq), dim3(256), 0, s, static_cast<const mx4_key *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
 			                   l < p.levels ? mid : last, over);
 		else
-			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4Gather>), dim3(nq), dim3(256), 0, s, a.lists, a.counts, a.parts, best, nbest, nq, k,
+			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4Gather, Mx4Record, 1, 4>), dim3(nq), dim3(256), 0, s, static_cast<const Mx4Record *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
 			                   l < p.levels ? mid : last, over);
 	}
 	if (p.levels)
