@@ -588,17 +588,28 @@ __device__ __forceinline__ void mx4_store_counts(const Mx4Queries<KS, C> &w, con
 		if (q0 + c * 32 + r32 < a.nq) a.counts[(int64_t)(q0 + c * 32 + r32) * a.parts + part] = a.list - 1 - (int)((w.last[c] - w.at[c]) / sizeof(R));
 }
 
-// Test of a lane's 16 products with each of its queries: the largest of every four, and whether any may be a candidate.
+// the largest of four neighbouring products, and `top` and four more: one after the other, which is two instructions (v_max3_f32), where a tree of
+// them is four to six (two, and the operands of the pairs made canonical)
+__device__ __forceinline__ float mx4_most(float top, const mx4_v16f &acc, int g)
+{
+	return __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(top, acc[4 * g]), acc[4 * g + 1]), acc[4 * g + 2]), acc[4 * g + 3]);
+}
+__device__ __forceinline__ float mx4_most(const mx4_v16f &acc, int g)
+{
+	return __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(acc[4 * g], acc[4 * g + 1]), acc[4 * g + 2]), acc[4 * g + 3]);
+}
+
+// Test of a lane's 16 products with each of its queries: the largest, and whether any may be a candidate.
 template <int KS, int C>
-__device__ __forceinline__ bool mx4_test(const Mx4Queries<KS, C> &w, const mx4_v16f (&acc)[C], float (&m)[C][4])
+__device__ __forceinline__ bool mx4_test(const Mx4Queries<KS, C> &w, const mx4_v16f (&acc)[C], float (&top)[C])
 {
 	bool any = false;
 #pragma unroll
 	for (int c = 0; c < C; c++) {
+		top[c] = mx4_most(acc[c], 0);
 #pragma unroll
-		for (int g = 0; g < 4; g++)
-			m[c][g] = __builtin_fmaxf(__builtin_fmaxf(acc[c][4 * g], acc[c][4 * g + 1]), __builtin_fmaxf(acc[c][4 * g + 2], acc[c][4 * g + 3]));
-		any |= __builtin_fmaxf(__builtin_fmaxf(m[c][0], m[c][1]), __builtin_fmaxf(m[c][2], m[c][3])) >= w.bound[c];
+		for (int g = 1; g < 4; g++) top[c] = mx4_most(top[c], acc[c], g);
+		any |= top[c] >= w.bound[c];
 	}
 	return any;
 }
@@ -616,19 +627,21 @@ __device__ __forceinline__ void mx4_append_one(Mx4Queries<KS, C> &w, const Mx4Le
 // mx4_pick_kernel.  Records take fewer instructions here, where they keep the matrix instructions waiting, and more there (1 M rows x 384, k 100:
 // 1000 queries 316 us with keys, 288 with records); with few queries a wave has few candidates and mx4_pick_kernel many lists (64 queries: 104 and 127).
 template <typename R, int KS, int C>
-__device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], const float (&m)[C][4], int64_t row0, int half)
+__device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level &a, const mx4_v16f (&acc)[C], const float (&top)[C], int64_t row0, int half)
 {
 	unsigned id0 = (unsigned)row0 + 4 * half;
 	asm volatile("" : "+v"(id0));  // the ids are formed here, where they are rarely wanted, not in the caller's loop
 #pragma unroll
-	for (int c = 0; c < C; c++)
+	for (int c = 0; c < C; c++) {
+		if (!__ballot(top[c] >= w.bound[c])) continue;
 #pragma unroll
-		for (int g = 0; g < 4; g++)
-			if (__ballot(m[c][g] >= w.bound[c])) {
+		for (int g = 0; g < 4; g++) {
+			const float m = mx4_most(acc[c], g);
+			if (__ballot(m >= w.bound[c])) {
 				if constexpr (sizeof(R) == sizeof(Mx4Record)) {
 					// (an equal product behind the bound's id is no candidate: rows that are all alike fill no lists)
 					const unsigned id = id0 + 8 * g;
-					if ((m[c][g] > w.bound[c]) | ((m[c][g] >= w.bound[c]) & (~id > (unsigned)w.bkey[c])))
+					if ((m > w.bound[c]) | ((m >= w.bound[c]) & (~id > (unsigned)w.bkey[c])))
 						mx4_append_one(w, a, c, Mx4Record{{acc[c][4 * g], acc[c][4 * g + 1], acc[c][4 * g + 2], acc[c][4 * g + 3]}, id});
 				} else {
 #pragma unroll
@@ -642,6 +655,8 @@ __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level 
 					}
 				}
 			}
+		}
+	}
 }
 
 // fragments of 32 queries a wave of the stream kernel holds
@@ -679,8 +694,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 		mx4_shift_scales(f, half);
 		mx4_v16f acc[C];
 		mx4_tile<KS, C>(f, w.b, acc);
-		float m[C][4];
-		if (__builtin_expect(__ballot(mx4_test(w, acc, m)) != 0, 0)) mx4_append<mx4_key>(w, a, acc, m, row0, half);
+		float top[C];
+		if (__builtin_expect(__ballot(mx4_test(w, acc, top)) != 0, 0)) mx4_append<mx4_key>(w, a, acc, top, row0, half);
 	};
 	if constexpr (KS <= 12) {
 		Mx4Frag<KS> f0, f1;
@@ -787,12 +802,12 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		mx4_shift_scales(f, half);
 		if constexpr (!PIPED) {
 			mx4_tile<KS, 2>(f, w.b, now);
-			float m[2][4];
-			if (__builtin_expect(__ballot(mx4_test(w, now, m)) != 0, 0)) mx4_append<Mx4Record>(w, a, now, m, row, half);
+			float top[2];
+			if (__builtin_expect(__ballot(mx4_test(w, now, top)) != 0, 0)) mx4_append<Mx4Record>(w, a, now, top, row, half);
 			return;
 		}
 		const mx4_v16f zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-		float m[2][4];
+		float top[2];
 #pragma unroll
 		for (int s = 0; s < KS; s++) {
 #pragma unroll
@@ -805,7 +820,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 #pragma unroll
 			for (int p = s * 8 / KS; p < (s + 1) * 8 / KS; p++) {  // a share of the test behind every two matrix instructions
 				const int c = p >> 2, g = p & 3;
-				m[c][g] = __builtin_fmaxf(__builtin_fmaxf(then[c][4 * g], then[c][4 * g + 1]), __builtin_fmaxf(then[c][4 * g + 2], then[c][4 * g + 3]));
+				top[c] = g == 0 ? mx4_most(then[c], 0) : mx4_most(top[c], then[c], g);
 			}
 			__builtin_amdgcn_sched_barrier(0);
 		}
@@ -813,8 +828,8 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		for (int c = 0; c < 2; c++) asm volatile("" : "+v"(now[c]));  // see mx4_tile
 		bool any = false;
 #pragma unroll
-		for (int c = 0; c < 2; c++) any |= __builtin_fmaxf(__builtin_fmaxf(m[c][0], m[c][1]), __builtin_fmaxf(m[c][2], m[c][3])) >= w.bound[c];
-		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append<Mx4Record>(w, a, then, m, row, half);
+		for (int c = 0; c < 2; c++) any |= top[c] >= w.bound[c];
+		if (__builtin_expect(__ballot(any) != 0, 0)) mx4_append<Mx4Record>(w, a, then, top, row, half);
 	};
 	for (int t = 0; t < ntiles; t += G) {
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the group is there ...
@@ -841,8 +856,8 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the tiles are done before it passes the next barrier
 	}
 	if (PIPED) {
-		float m[2][4];
-		if (__ballot(mx4_test(w, accB, m))) mx4_append<Mx4Record>(w, a, accB, m, rowB, half);
+		float top[2];
+		if (__ballot(mx4_test(w, accB, top))) mx4_append<Mx4Record>(w, a, accB, top, rowB, half);
 	}
 	mx4_store_counts<Mx4Record>(w, a, q0, 2 * split + half, r32);
 }
