@@ -298,7 +298,7 @@ def test_scan_many_queries(engines):
     _check_scan(engines(64), M.pack(_unit(rng, 8200, 64)), M.pack(_unit(rng, 3300, 64)), 3)
 
 
-@pytest.mark.parametrize("nq", [1, 70])
+@pytest.mark.parametrize("nq", [1, 70, 300])
 def test_scan_leaves_out_nan(engines, nq):
     rng = np.random.default_rng(nq)
     x = _unit(rng, 5000, 100)
@@ -322,6 +322,11 @@ def test_scan_infinite_products(engines):
     v = val.cpu().numpy()
     assert (cnt.cpu().numpy() == 128).all() and np.isposinf(v[:, :100]).all() and np.isfinite(v[:, 100:]).all()
     assert np.array_equal(ids.cpu().numpy()[0, :100], np.arange(0, 300, 3)) and np.array_equal(ids.cpu().numpy()[1, :100], np.arange(1, 300, 3))
+    for nq in (40, 300):  # in levels, the infinite ones late
+        ids, val, cnt = engines(64).scan_many(_to(M.pack(np.repeat(q, nq // 2, 0))), _to(M.pack(np.concatenate([np.zeros((6000, 64), np.float32), x]))), 128)
+        v, i = val.cpu().numpy(), ids.cpu().numpy()
+        assert (cnt.cpu().numpy() == 128).all() and np.isposinf(v[:, :100]).all() and np.isfinite(v[:, 100:]).all()
+        assert (i[: nq // 2, :100] == np.arange(6000, 6300, 3)).all() and (i[nq // 2 :, :100] == np.arange(6001, 6300, 3)).all()
 
 
 @pytest.mark.parametrize("nq,n,dim", [(3, 4000, 384), (200, 9000, 1024)])
