@@ -5,7 +5,7 @@
 // and rows whose product is NaN are no candidates; a row is taken out by giving its blocks the scale 255, which makes every product NaN,
 // and a NaN is never >= a bound.
 //
-// Two ways, by the number of queries (1 M rows x 384, k 10: 8 queries 56 us in chunks, 9 queries 75 us in levels, 64 queries 79 us):
+// Two ways, by the number of queries (1 M rows x 384, k 10: 8 queries 56 us in chunks, 9 queries 71 us in levels, 64 queries 79 us):
 //
 // CHUNKS (up to 8 queries): a workgroup computes the products of its own run of rows, keeps them in LDS and picks the best k of each
 // query there; a second launch picks the best k of those.  Every row is read once, and two launches are all there is.
@@ -283,7 +283,8 @@ __device__ void mx4_block_leave(int have, int k, mx4_key *dst, Mx4PickLds &l)
 	}
 }
 
-// one workgroup per query: the best k of the `m` keys that the chunks left (0 = none), 7 x 1024 at a time beside the best so far
+// one workgroup per query: the best k of the `m` keys that the chunks left (0 = none), 7 x 1024 at a time beside the best so far.  Bound by its steps,
+// each of which waits for the one before: 4.6 us for 4890 keys
 __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *keys, int m, int k, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
@@ -303,7 +304,6 @@ __global__ __launch_bounds__(1024) void mx4_pick_chunks_kernel(const mx4_key *ke
 	mx4_block_put<1024>(have, k, q, o, l);
 }
 
-// T threads per query (a workgroup, or a wave of one): the best k of what it had and of its lists, CAP keys in all
 // What a list holds: keys, or (many queries) records of four neighbouring rows of which at least one may be a candidate: the first one's id, and the
 // products (NaN: a row that does not count).
 struct __attribute__((packed, aligned(4))) Mx4Record {
@@ -322,6 +322,9 @@ __device__ __forceinline__ void mx4_keys_of(const Mx4Record &r, mx4_key (&key)[4
 constexpr int kMx4Gather = 2048, kMx4GatherFewQueries = 4096;
 constexpr int kMx4GatherWave = 768;  // the most that a wave deals with
 
+// T threads per query (a workgroup, or a wave of one): the best k of what it had and of its lists, CAP keys in all.  Bound by its steps, each of
+// which waits for the one before: 14 us for 333 queries with 512 lists and 1000 keys each, 9 us for 1000 with 256 and 90, 13 us for 4096 with 32 and 90
+// (a wave each).
 template <int T, int CAP, typename R, int LISTS, int P>
 __global__ __launch_bounds__(256) void mx4_pick_kernel(const R *lists, const int32_t *counts, int parts, int list, const mx4_key *before,
                                                        const int32_t *nbefore, const mx4_key *bound, int nq, int k, Mx4Out o, int32_t *over)
@@ -436,7 +439,9 @@ constexpr int64_t kMx4ChunkKeys = 1 << 17;  // keys that the chunks leave for a 
 static_assert(kMx4ChunkThreads / 64 >= kMx4ChunkQ, "a wave for each query");
 
 // A wave takes 32 rows at a time, the next ones on their way meanwhile.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
-// quarters of the matrix work is for nothing: it is a few us at a million rows, against the reading of them.
+// quarters of the matrix work is for nothing: it is a few us at a million rows, against the reading of them:
+// 33.6 us for 1 M x 384 and one query, 6.2 TB/s.  As level 0 of many queries every workgroup reads the same 2048 rows, 16 bytes of a row a lane, and is
+// bound by what the address path takes, about a lane a cycle: 21 us for 1000 queries, 45 us for 4096 (x 512).
 template <int KS>
 __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int k, int chunk,
                                                                      const uint32_t *allow, mx4_key *out, int64_t stride, int64_t step, Mx4Out o,
@@ -562,7 +567,7 @@ struct Mx4Queries {
 	Mx4Frag<KS> b[C];
 	float bound[C];
 	mx4_key bkey[C];
-	unsigned at[C], last[C];  // byte offsets of the list's next place and of its last
+	unsigned at[C], last[C];  // byte offsets of the list's next place and of its last (at most 262 144 lists of a few KB: mx4_plan)
 };
 
 template <typename R, int KS, int C>
@@ -662,8 +667,9 @@ __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level 
 // fragments of 32 queries a wave of the stream kernel holds
 __host__ __device__ constexpr int mx4_stream_frags(int ks) { return ks <= 8 ? 2 : 1; }
 
-// Independent waves: each holds 64 queries (32 where rows are long) and takes every (waves)-th half tile of the level straight from memory, the next one's rows under
-// way while it multiplies.
+// Independent waves: each holds 64 queries (32 where rows are long) and takes every (waves)-th half tile of the level straight from memory, the next
+// one's rows under way while it multiplies.  Bound by the reading of the rows up to 64 queries (9 queries: the last level of 1 M x 384 in 30 us), above
+// by their reading once for every 64: 256 queries 76 us, where tiles shared in LDS take as long and cost more at their start.
 template <int KS>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgroups)
 {
@@ -732,7 +738,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 // worked on the tiles of the next are asked for, one after the other.  One barrier a group: a wave that appends keeps the others waiting there, the
 // less the further the barriers are apart (4096 queries, 900 000 x 512, 168 candidates a query: barriers 1 tile apart 960 us, 2 tiles 880 us).
 // An image row is the packed row, plus one slot of 16 bytes where that makes the stride an odd number of slots: then the 16 lanes that an LDS read
-// serves at a time hit 16 different slots.  Two waves a SIMD.
+// serves at a time hit 16 different slots.  Two waves a SIMD.  4096 queries, 900 000 x 512: 725 us, 5.2 PFLOP/s (this card sustains 6.6 on random
+// operands); 1000 queries, x 384: 166 us, 4.2 PFLOP/s.
 static __device__ __align__(16) int g_mx4_nan[4] = {-1, -1, -1, -1};  // scales 255: the blocks of a row that is left out
 
 __host__ __device__ constexpr int mx4_image_slots(int row_bytes) { return (row_bytes / 16) | 1; }
@@ -862,13 +869,18 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	mx4_store_counts<Mx4Record>(w, a, q0, 2 * split + half, r32);
 }
 
+// (by value: `first ? x[1] : x[0]` is a place in memory)
+__device__ __forceinline__ float mx4_select(bool first, float a, float b) { return first ? a : b; }
+
 // The queries that lost keys, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
-// to the best k when the next 128 might not fit.
+// to the best k when the next 128 might not fit; from then on what is below all that were kept is none.  Bound by its steps, 0.6 us for
+// 128 rows (300 queries, 96 000 x 64, all of them done over: 0.46 ms; without that bound, and one lane going through the products, 2.98 ms).
 template <int KS>
 __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, const int32_t *over, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
 	__shared__ mx4_key keys[kMx4Gather];
+	__shared__ mx4_key least;  // of those that were kept, if that is k
 	__shared__ int count;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, r32 = lane & 31;
 	for (int q = blockIdx.x; q < a.nq; q += gridDim.x) {
@@ -877,26 +889,33 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 		mx4_load_frag<KS>(b[0], a.q + (int64_t)q * mx4_row_bytes(64 * KS), half);
 		mx4_shift_scales(b[0], half);
 		int have = 0;
-		if (tid == 0) count = 0;
+		if (tid == 0) {
+			count = 0;
+			least = 0;
+		}
 		__syncthreads();
+		auto load = [&](int64_t row0, Mx4Frag<KS> &f) {
+			const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
+			mx4_load_frag<KS>(f, a.rows + r * mx4_row_bytes(64 * KS), half);
+		};
+		Mx4Frag<KS> f, next;
+		load(wave * 32, next);
 		for (int64_t base = 0; base < a.n; base += 128) {
 			const int64_t row0 = base + wave * 32;
+			f = next;
+			load(row0 + 128, next);
 			if (row0 < a.n) {
-				const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
-				Mx4Frag<KS> f;
-				mx4_load_frag<KS>(f, a.rows + r * mx4_row_bytes(64 * KS), half);
 				mx4_shift_scales(f, half);
 				mx4_v16f acc[1];
 				mx4_tile<KS, 1>(f, b, acc);
-				if (r32 == 0) {  // every column holds the same query
+				// every column holds the same query: column i < 16 deals with the i-th of its products
+				float v = acc[0][0];
 #pragma unroll
-					for (int i = 0; i < 16; i++) {
-						const int64_t id = row0 + 8 * (i >> 2) + 4 * half + (i & 3);
-						if (id < a.n && (!a.allow || ((a.allow[id >> 5] >> (id & 31)) & 1u))) {
-							const mx4_key key = mx4_make_key(acc[0][i], (unsigned)id);
-							if (key) keys[atomicAdd(&count, 1)] = key;
-						}
-					}
+				for (int i = 1; i < 16; i++) v = mx4_select(r32 == i, acc[0][i], v);
+				const int64_t id = row0 + 8 * (r32 >> 2) + 4 * half + (r32 & 3);
+				if (r32 < 16 && id < a.n && (!a.allow || ((a.allow[id >> 5] >> (id & 31)) & 1u))) {
+					const mx4_key key = mx4_make_key(v, (unsigned)id);
+					if (key > least) keys[atomicAdd(&count, 1)] = key;
 				}
 			}
 			__syncthreads();
@@ -905,9 +924,16 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 #pragma unroll
 				for (int j = 0; j < kMx4Gather / 256; j++) key[j] = j * 256 + tid < count ? keys[j * 256 + tid] : 0;
 				__syncthreads();
+				if (tid == 0) least = ~(mx4_key)0;
 				have = mx4_block_best<256>(key, k, l);
-				for (int j = tid; j < have; j += 256) keys[j] = l.best[j];
-				if (tid == 0) count = have;
+				for (int j = tid; j < have; j += 256) {
+					keys[j] = l.best[j];
+					if (have >= k) atomicMin(&least, l.best[j]);
+				}
+				if (tid == 0) {
+					count = have;
+					if (have < k) least = 0;
+				}
 			}
 			__syncthreads();
 		}
@@ -1078,15 +1104,17 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 			hipLaunchKernelGGL((mx4_stage_kernel<KS>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
 		else
 			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
+		const Mx4Out &out = l < p.levels ? mid : last;
+		auto pick = [&](auto kernel, auto record, int groups) {
+			hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, s, static_cast<const decltype(record) *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound,
+			                   nq, k, out, over);
+		};
 		if (p.few)
-			hipLaunchKernelGGL((mx4_pick_kernel<64, kMx4GatherWave, Mx4Record, 1, 4>), dim3((nq + 3) / 4), dim3(256), 0, s, static_cast<const Mx4Record *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
-			                   l < p.levels ? mid : last, over);
-		else if (!stage)
-			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4GatherFewQueries, mx4_key, 4, 2>), dim3(nq), dim3(256), 0, s, static_cast<const mx4_key *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
-			                   l < p.levels ? mid : last, over);
+			pick(mx4_pick_kernel<64, kMx4GatherWave, Mx4Record, 1, 4>, Mx4Record{}, (nq + 3) / 4);
+		else if (stage)
+			pick(mx4_pick_kernel<256, kMx4Gather, Mx4Record, 1, 4>, Mx4Record{}, nq);
 		else
-			hipLaunchKernelGGL((mx4_pick_kernel<256, kMx4Gather, Mx4Record, 1, 4>), dim3(nq), dim3(256), 0, s, static_cast<const Mx4Record *>(a.lists), a.counts, a.parts, a.list, best, nbest, bound, nq, k,
-			                   l < p.levels ? mid : last, over);
+			pick(mx4_pick_kernel<256, kMx4GatherFewQueries, mx4_key, 4, 2>, mx4_key{}, nq);
 	}
 	if (p.levels)
 		hipLaunchKernelGGL((mx4_rescue_kernel<KS>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
