@@ -440,8 +440,8 @@ static_assert(kMx4ChunkThreads / 64 >= kMx4ChunkQ, "a wave for each query");
 
 // A wave takes 32 rows at a time, the next ones on their way meanwhile.  Queries are the columns of D, so with nq <= 8 of 32 columns used three
 // quarters of the matrix work is for nothing: it is a few us at a million rows, against the reading of them:
-// 33.6 us for 1 M x 384 and one query, 6.2 TB/s.  As level 0 of many queries every workgroup reads the same 2048 rows, 16 bytes of a row a lane, and is
-// bound by what the address path takes, about a lane a cycle: 21 us for 1000 queries, 45 us for 4096 (x 512).
+// 33.6 us for 1 M x 384 and one query, 6.2 TB/s.  As level 0 of many queries every workgroup reads the same 2048 rows, 16 bytes of a row a lane, which
+// fits an address path that takes a lane a cycle (counted, not measured): 21 us for 1000 queries, 45 us for 4096 (x 512).
 template <int KS>
 __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int k, int chunk,
                                                                      const uint32_t *allow, mx4_key *out, int64_t stride, int64_t step, Mx4Out o,
