@@ -10,12 +10,16 @@
 // CHUNKS (up to 8 queries): a workgroup computes the products of its own run of rows, keeps them in LDS and picks the best k of each
 // query there; a second launch picks the best k of those.  Every row is read once, and two launches are all there is.
 //
-// LEVELS (more): the rows are taken in levels of 64-row tiles, each about `ratio` times the one before it: level 0 is every
-// ratio^L-th tile, level l the tiles that are multiples of ratio^(L - l) and not of ratio^(L - l + 1).  After a level the k-th best key so
-// far is a bound: k rows are at least that good, so only keys above it matter, and as the rows seen so far are spread evenly over the
-// store about k (ratio - 1) keys of the next level are (whatever order the rows are in, unless they repeat with the tiles' period).
+// LEVELS (more): the 64-row tiles are taken in levels, each about `ratio` times the one before it.  All tiles stand in one order, tile
+// p of it being tile (p M) mod T of the T there are, M near T / golden ratio and without a common divisor, and a level is a run of that order.
+// The tiles seen up to any level are spread evenly over the store (mx4_spread), and a layout that repeats every so many tiles (pages dealt out
+// in turn to tenants, one of which the filter keeps) is met at about its share in every level, where tiles at equal distances see all of it or nothing:
+// 1 M x 384, every 8th tile allowed, 300 queries take 146 us, at equal distances 8.4 ms.  (Counted over 300 stores of up to 40 000 tiles and periods of up to
+// 128: 1 to 2 % of the pairs are still too much for a level's lists, 15 to 21 % at equal distances.)  The price is 1 % at 4096 queries x 1 M x
+// 512 and 3 % at 40 M rows, 8 GB that are no longer read from end to end.  After a level the k-th best key so far is a bound: k rows are at least that good,
+// so only keys above it matter, and about k (ratio - 1) keys of the next level are, unless the next level is better than what was seen.
 // Level 0 has no bound: it is one chunk.  From then on a lane whose product passes the bound appends it to a list of its own,
-// which needs no atomics: a lane only ever sees one query a fragment, and the tiles are dealt out in turn, so lists stay short.
+// which needs no atomics: a lane only ever sees one query a fragment, and what it takes at a stretch of the order lies far apart, so lists stay short.
 // mx4_pick_kernel gathers a query's lists after every level and keeps the best k.  A list that overflows marks its query, and
 // mx4_rescue_kernel does those over, one workgroup each.
 #pragma once
@@ -318,7 +322,7 @@ __device__ __forceinline__ void mx4_keys_of(const Mx4Record &r, mx4_key (&key)[4
 }
 
 // Keys of all lists of a query.  The plan sees to it that a random order of the rows stays far below them; what asks for more is a run of neighbouring
-// rows that are all candidates and that the levels before have missed, at most 64 x ratio of them.
+// rows that are all candidates and that the levels before have missed, at most about 64 x 2.7 ratio of them.
 constexpr int kMx4Gather = 2048, kMx4GatherFewQueries = 4096;
 constexpr int kMx4GatherWave = 768;  // the most that a wave deals with
 
@@ -431,6 +435,37 @@ __device__ __forceinline__ void mx4_tile(const Mx4Frag<KS> &a, const Mx4Frag<KS>
 	for (int c = 0; c < C; c++) asm volatile("" : "+v"(acc[c]));
 }
 
+// ---------------------------------------------------------------------------------------------- the order of the tiles
+// Tile at place p of the order, (p M) mod T, from spread = ceil(2^64 M / T): p spread = 2^64 p M / T + e p with 0 <= e < 1, so its lower 64 bits are
+// 2^64 ((p M) mod T) / T + e p, and times T / 2^64 that is (p M) mod T + e p T / 2^64: less than 1 more, as p and T are at most 2^25.
+__device__ __forceinline__ unsigned mx4_tile_at(uint64_t spread, unsigned tiles, unsigned p)
+{
+	return (unsigned)__umul64hi(p * spread, (uint64_t)tiles);
+}
+// The tiles up to any place leave no gap of more than 2.7 times the mean one as long as the continued fraction of M / T has no large term.  The fraction
+// of the golden ratio has none, but that of a whole M beside T / golden ratio is like it only in its first half: the first M from there on whose terms are
+// at most 5 (6 are tried on average, 64 at most: then the best of them, of 7 in the worst of 300 T up to 40 000).  T >= 2.
+inline uint64_t mx4_spread(uint32_t tiles)
+{
+	const uint32_t from = (uint32_t)(0.6180339887498949 * tiles);
+	uint32_t best = 1, best_term = ~0u;
+	for (uint32_t i = 0; i < 64 && best_term > 5; i++) {
+		const uint32_t m = (i & 1) ? from - (i + 1) / 2 : from + i / 2;
+		if (m == 0 || m >= tiles) continue;  // (what wraps below 0 is large)
+		uint32_t a = tiles, b = m, term = 0;
+		while (b) {
+			const uint32_t t = a / b, c = a - t * b;
+			term = t > term ? t : term;
+			a = b;
+			b = c;
+		}
+		if (a != 1 || term >= best_term) continue;
+		best = m;
+		best_term = term;
+	}
+	return (uint64_t)((((unsigned __int128)best << 64) + tiles - 1) / tiles);
+}
+
 // ---------------------------------------------------------------------------------------------- chunks
 constexpr int kMx4ChunkQ = 8;        // queries of a workgroup
 constexpr int kMx4ChunkRows = 2048;  // rows a workgroup, at most
@@ -444,24 +479,24 @@ static_assert(kMx4ChunkThreads / 64 >= kMx4ChunkQ, "a wave for each query");
 // fits an address path that takes a lane a cycle (counted, not measured): 21 us for 1000 queries, 45 us for 4096 (x 512).
 template <int KS>
 __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8_t *q, int nq, const uint8_t *rows, int n, int k, int chunk,
-                                                                     const uint32_t *allow, mx4_key *out, int64_t stride, int64_t step, Mx4Out o,
-                                                                     int32_t *over, int qper)
+                                                                     const uint32_t *allow, mx4_key *out, int64_t stride, uint64_t spread,
+                                                                     unsigned tiles, Mx4Out o, int32_t *over, int qper)
 {
 	extern __shared__ __attribute__((aligned(16))) float sc[];  // [nq][chunk]
 	__shared__ Mx4PickLds l[kMx4ChunkQ];
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, r32 = lane & 31;
 	const int64_t first = (int64_t)blockIdx.x * chunk;
-	const int64_t end = step > 1 ? chunk : n - first;  // (tiles apart: the host gives as many as there are, the last may end early)
+	const int64_t end = spread ? chunk : n - first;  // (tiles apart: the host gives as many as there are, one may end early)
 	const int m = (int)(end < chunk ? end : chunk);
 	const int qbase = blockIdx.y * qper;
 	q += (int64_t)qbase * row_bytes;
 	nq = nq - qbase < qper ? nq - qbase : qper;
-	// row of place t: rows in a run, or (step > 1, one workgroup for them all) the 64-row tiles that are multiples of step
-	auto row_of = [&](int t) -> int64_t { return first + t + (int64_t)(t & ~63) * (step - 1); };
+	// row of place t, a multiple of 64 that all lanes agree on: rows in a run, or (spread, one workgroup for them all) the first tiles of the order
+	auto row_of = [&](int t) -> int64_t { return spread ? (int64_t)mx4_tile_at(spread, tiles, (unsigned)t >> 6) * 64 : first + t; };
 	Mx4Frag<KS> b[1], f0, f1;
 	auto load = [&](int t, Mx4Frag<KS> &f) {
-		const int64_t r = row_of(t + r32 < m ? t + r32 : m - 1);
+		const int64_t r = row_of(t & ~63) + (t & 32) + r32;
 		mx4_load_frag<KS>(f, rows + (r < n ? r : n - 1) * row_bytes, half);
 	};
 	auto use = [&](int t, Mx4Frag<KS> &f) {
@@ -510,7 +545,7 @@ __global__ __launch_bounds__(kMx4ChunkThreads) void mx4_chunk_kernel(const uint8
 			const int at = j * T + (tid & (T - 1));
 			key[j] = 0;
 			if (j * T >= m) continue;
-			const int64_t id = row_of(at);
+			const int64_t id = row_of(j * T + (T > 64 ? wave * 64 : 0)) + lane;
 			const bool in = at < m && id < n && (!allow || ((allow[id >> 5] >> (id & 31)) & 1u));
 			key[j] = in ? mx4_make_key(sc[qi * chunk + at], (unsigned)id) : 0;
 		}
@@ -538,21 +573,19 @@ struct Mx4Level {
 	const uint8_t *q, *rows;
 	const uint32_t *allow;
 	int nq, n;
-	int64_t step;     // see mx4_tile_row
-	uint64_t skip;    // ceil(2^32 / (ratio - 1)); 0: every multiple of step is a tile of the level
-	int tiles;
+	uint64_t spread;  // see mx4_tile_at
+	unsigned all;     // tiles of the store
+	unsigned first;   // place of the level's first tile in the order
+	int each, more;   // tiles in a row that a wave pair (stream) or workgroup (stage) takes, the first `more` of them one more: tiles of
+	                  // neighbouring rows, which may all hold candidates, are far apart in the order, so they go to different lists
 	const mx4_key *bound;  // [nq], 0 = none
 	void *lists;       // [nq][parts][list] keys or records
 	int32_t *counts;   // [nq][parts] how many a list holds; list - 1: some may be lost
 	int parts, list;
 };
 
-// tile i of a level, first row: i / (ratio - 1) by a multiplication, exact for i (ratio - 1) < 2^32 (i < 2^25)
-__device__ __forceinline__ int64_t mx4_tile_row(const Mx4Level &a, unsigned i)
-{
-	if (a.skip) i += (unsigned)((i * a.skip) >> 32) + 1;
-	return (int64_t)i * a.step * 64;
-}
+// tile i of a level, first row
+__device__ __forceinline__ int64_t mx4_tile_row(const Mx4Level &a, unsigned i) { return (int64_t)mx4_tile_at(a.spread, a.all, a.first + i) * 64; }
 
 // a word of the filter at a place that all lanes agree on, through the scalar cache (a vector load would wait for the LDS-DMA loads before it)
 __device__ __forceinline__ uint32_t mx4_allow_word(const uint32_t *allow, int64_t at)
@@ -667,23 +700,23 @@ __device__ __forceinline__ void mx4_append(Mx4Queries<KS, C> &w, const Mx4Level 
 // fragments of 32 queries a wave of the stream kernel holds
 __host__ __device__ constexpr int mx4_stream_frags(int ks) { return ks <= 8 ? 2 : 1; }
 
-// Independent waves: each holds 64 queries (32 where rows are long) and takes every (waves)-th half tile of the level straight from memory, the next
+// Independent waves: each holds 64 queries (32 where rows are long) and takes its half of a run of the level's tiles straight from memory, the next
 // one's rows under way while it multiplies.  Bound by the reading of the rows up to 64 queries (9 queries: the last level of 1 M x 384 in 30 us), above
 // by their reading once for every 64: 256 queries 76 us, where tiles shared in LDS take as long and cost more at their start.
 template <int KS>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgroups)
 {
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
-	const int gw = blockIdx.x * 4 + wave, group = gw % qgroups, waves = a.parts / 2, first = gw / qgroups;
-	if (first >= waves) return;
+	const int gw = blockIdx.x * 4 + wave, group = gw % qgroups, first = gw / qgroups;
+	if (first >= a.parts / 2) return;
 	constexpr int row_bytes = mx4_row_bytes(64 * KS);
 	constexpr int C = mx4_stream_frags(KS);
 	Mx4Queries<KS, C> w;
 	mx4_load_queries<mx4_key>(w, a, group * 32 * C, 2 * first + half, half, r32);
-	const unsigned total = 2 * (unsigned)a.tiles;
-	// half tile i: its first row and which of its rows count, and (unless none does) the rows
-	auto load = [&](unsigned i, Mx4Frag<KS> &f, int64_t &row0, unsigned &keep) {
-		row0 = mx4_tile_row(a, i >> 1) + (i & 1) * 32;
+	const int pair = first >> 1, from = pair * a.each + (pair < a.more ? pair : a.more), total = a.each + (pair < a.more ? 1 : 0);
+	// this wave's half of the pair's tile i: its first row and which of its rows count, and (unless none does) the rows
+	auto load = [&](int i, Mx4Frag<KS> &f, int64_t &row0, unsigned &keep) {
+		row0 = mx4_tile_row(a, from + i) + (first & 1) * 32;
 		keep = 0;
 		if (row0 >= a.n) return;
 		keep = row0 + 32 <= a.n ? 0xffffffffu : (1u << (a.n - row0)) - 1u;
@@ -707,23 +740,22 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 		Mx4Frag<KS> f0, f1;
 		int64_t row0, row1;
 		unsigned keep0 = 0, keep1 = 0;
-		unsigned i = first;
+		int i = 0;
 		if (i < total) load(i, f0, row0, keep0);
 		while (i < total) {
 			keep1 = 0;
-			if (i + waves < total) load(i + waves, f1, row1, keep1);
+			if (i + 1 < total) load(i + 1, f1, row1, keep1);
 			__builtin_amdgcn_sched_barrier(0);
 			use(f0, row0, keep0);
-			i += waves;
-			if (i >= total) break;
+			if (++i >= total) break;
 			keep0 = 0;
-			if (i + waves < total) load(i + waves, f0, row0, keep0);
+			if (i + 1 < total) load(i + 1, f0, row0, keep0);
 			__builtin_amdgcn_sched_barrier(0);
 			use(f1, row1, keep1);
-			i += waves;
+			i++;
 		}
 	} else {
-		for (unsigned i = first; i < total; i += waves) {
+		for (int i = 0; i < total; i++) {
 			Mx4Frag<KS> f;
 			int64_t row0;
 			unsigned keep;
@@ -749,7 +781,7 @@ __host__ __device__ constexpr int mx4_stage_group(int ks) { return ks <= 8 ? 4 :
 __host__ __device__ constexpr size_t mx4_stage_lds(int ks) { return (size_t)2 * mx4_stage_group(ks) * mx4_image_slots(mx4_row_bytes(64 * ks)) * 1024; }
 
 template <int KS>
-__global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtiles, int splits)
+__global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtiles)
 {
 	extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r32 = lane & 31;
@@ -764,13 +796,13 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 	const int q0 = (qtile * nwaves + wave) * 64;
 	Mx4Queries<KS, 2> w;
 	mx4_load_queries<Mx4Record>(w, a, q0, 2 * split + half, half, r32);
-	const int ntiles = split < a.tiles ? (a.tiles - split + splits - 1) / splits : 0;
+	const int from = split * a.each + (split < a.more ? split : a.more), ntiles = a.each + (split < a.more ? 1 : 0);
 
 	using lds_ptr_t = __attribute__((address_space(3))) void *;
 	using glb_ptr_t = __attribute__((address_space(1))) const void *;
 	// this wave's share of tile t: instructions wave, wave + nwaves, ... of islots, 64 slots of 16 bytes each
 	auto fetch = [&](int t) {
-		const int64_t row0 = mx4_tile_row(a, split + t * splits);
+		const int64_t row0 = mx4_tile_row(a, from + t);
 		const uint8_t *base = a.rows + row0 * row_bytes;
 		unsigned char *dst = lds + (t & (2 * G - 1)) * tile_bytes;
 		if (islots == slots && !a.allow && row0 + 64 <= a.n) {  // the image is the tile as it lies in memory
@@ -845,7 +877,7 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 		if (AHEAD) mx4_load_frag<KS>(f0, image(t, 0), half);
 		for (int u = t; u < t + G && u < ntiles; u++) {
 			if (u + G < ntiles) fetch(u + G);
-			const int64_t row0 = mx4_tile_row(a, split + u * splits);
+			const int64_t row0 = mx4_tile_row(a, from + u);
 			if (!AHEAD) mx4_load_frag<KS>(f0, image(u, 0), half);
 			if (AHEAD) {
 				mx4_load_frag<KS>(f1, image(u, 1), half);
@@ -952,7 +984,7 @@ struct Mx4Plan {
 	bool chunks, few;  // few: keys that a query gathers in a level
 	int chunk, parts, list;  // chunks: rows of one, how many; levels: lists of a query, places of a list
 	int levels, ratio, first_rows;  // levels after level 0; rows of level 0 (a multiple of 64)
-	int64_t step0;
+	int64_t step0;  // ratio^levels: one in so many tiles is in level 0
 	int slab, qgroups, qtiles, splits, record;  // record: bytes of what a list holds
 	size_t ws;
 };
@@ -1002,7 +1034,7 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 		const int wide = 32 * mx4_stream_frags(mx4_blocks(dim) / 2);
 		p.qgroups = (p.slab + wide - 1) / wide;
 		const int64_t most_waves = kMx4StreamWaves / p.qgroups;
-		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 1) : most_waves);
+		p.splits = (int)(2 * tiles < most_waves ? (tiles ? 2 * tiles : 2) : most_waves & ~1);  // (waves, in pairs)
 	}
 	p.parts = 2 * p.splits;
 	// a list's share of a level's candidates, with the same margin, and room for neighbouring rows that are all candidates, three tiles of them in
@@ -1044,8 +1076,8 @@ hipError_t mx4_scan_chunks(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const hipError_t e = mx4_allow_lds(reinterpret_cast<const void *>(&mx4_chunk_kernel<KS>), kMx4ChunkQ * kMx4ChunkRows * 4, Mx4Mark<KS, 0>::set);
 	if (e != hipSuccess) return e;
 	if (p.parts > 0)
-		hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(p.parts, 1), dim3(kMx4ChunkThreads), lds, s, q, nq, rows, n, k, p.chunk, allow, keys, stride, (int64_t)1, Mx4Out{},
-		                   static_cast<int32_t *>(nullptr), kMx4ChunkQ);
+		hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(p.parts, 1), dim3(kMx4ChunkThreads), lds, s, q, nq, rows, n, k, p.chunk, allow, keys, stride, (uint64_t)0,
+		                   0u, Mx4Out{}, static_cast<int32_t *>(nullptr), kMx4ChunkQ);
 	hipLaunchKernelGGL(mx4_pick_chunks_kernel, dim3(nq), dim3(1024), 0, s, keys, (int)stride, k, o);
 	return hipGetLastError();
 }
@@ -1073,6 +1105,8 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	a.bound = bound;
 	a.parts = p.parts;
 	if (p.levels) {
+		a.all = (unsigned)(((int64_t)n + 63) / 64);
+		a.spread = mx4_spread(a.all);
 		a.counts = static_cast<int32_t *>(take((size_t)p.slab * p.parts * 4));
 		a.list = p.list;
 		a.lists = take((size_t)p.slab * p.parts * p.list * p.record);
@@ -1092,16 +1126,16 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 	const int qper = nq >= 256 * kMx4ChunkQ ? kMx4ChunkQ : (nq + 255) / 256;  // a workgroup for every compute unit if there are queries enough
 	hipLaunchKernelGGL((mx4_chunk_kernel<KS>), dim3(1, (nq + qper - 1) / qper), dim3(kMx4ChunkThreads),
 	                   (size_t)qper * (p.first_rows ? p.first_rows : 64) * 4, s, q, nq, rows, n, k, p.first_rows, allow,
-	                   static_cast<mx4_key *>(nullptr), (int64_t)0, p.step0, p.levels ? mid : last, over, qper);
-	const int64_t tiles = ((int64_t)n + 63) / 64;
-	a.step = p.step0;
-	a.skip = p.ratio > 1 ? (((uint64_t)1 << 32) + p.ratio - 2) / (p.ratio - 1) : 0;
+	                   static_cast<mx4_key *>(nullptr), (int64_t)0, a.spread, a.all, p.levels ? mid : last, over, qper);
+	int64_t step = p.step0;
 	for (int l = 1; l <= p.levels; l++) {
-		const int64_t before = (tiles + a.step - 1) / a.step;
-		a.step /= p.ratio;
-		a.tiles = (int)((tiles + a.step - 1) / a.step - before);
+		a.first = (unsigned)((a.all + step - 1) / step);
+		step /= p.ratio;
+		const int tiles = (int)((a.all + step - 1) / step - a.first), takers = stage ? p.splits : p.splits / 2;
+		a.each = tiles / takers;
+		a.more = tiles % takers;
 		if (stage)
-			hipLaunchKernelGGL((mx4_stage_kernel<KS>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles, p.splits);
+			hipLaunchKernelGGL((mx4_stage_kernel<KS>), dim3(p.qtiles * p.splits), dim3(64 * nwaves), lds, s, a, p.qtiles);
 		else
 			hipLaunchKernelGGL((mx4_stream_kernel<KS>), dim3((unsigned)((p.splits * p.qgroups + 3) / 4)), dim3(256), 0, s, a, p.qgroups);
 		const Mx4Out &out = l < p.levels ? mid : last;
