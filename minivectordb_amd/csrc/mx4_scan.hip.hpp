@@ -905,9 +905,12 @@ __global__ __launch_bounds__(512, 2) void mx4_stage_kernel(Mx4Level a, int qtile
 __device__ __forceinline__ float mx4_select(bool first, float a, float b) { return first ? a : b; }
 
 // The queries that lost keys, from the beginning: a workgroup for each, 128 rows at a time, candidates gathered in LDS and cut
-// to the best k when the next 128 might not fit; from then on what is below all that were kept is none.  Bound by its steps, 0.6 us for
-// 128 rows (300 queries, 96 000 x 64, all of them done over: 0.46 ms; without that bound, and one lane going through the products, 2.98 ms).
-template <int KS>
+// to the best k when the next 128 might not fit; from then on what is below all that were kept is none.  Bound by its steps, 0.6
+// to 0.7 us for 128 rows (300 queries, 96 000 x 64, all of them done over: 0.46 ms; without that bound, and one lane going through the products,
+// 2.98 ms).  Beside queries that fit it is a cliff: one of 300 at 1 M x 384 makes 146 us 5.5 ms, all of them 6.0 ms.  With a filter groups of 128 rows none
+// of which may be returned are passed over (one page of 1024 rows in 8 allowed: 8.5 ms for all 300 without that, 1.5 ms with), and without one there is no
+// test for it (a test at run time instead of two kernels: 6.5 ms for the 6.0).
+template <int KS, bool FILTER>
 __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, const int32_t *over, Mx4Out o)
 {
 	__shared__ Mx4PickLds l;
@@ -930,12 +933,34 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 			const int64_t r = row0 + r32 < a.n ? row0 + r32 : a.n - 1;
 			mx4_load_frag<KS>(f, a.rows + r * mx4_row_bytes(64 * KS), half);
 		};
+		// With a filter, groups of 128 rows none of which may be returned are passed over: bit i of `some` says that group i of the 64 from row
+		// `from` on has one and has not been dealt with.
+		int64_t from = FILTER ? -64 * 128 : -128;
+		uint64_t some = 0;
+		auto step = [&]() -> int64_t {  // the next 128 rows, or past the last
+			if constexpr (!FILTER) return from += 128;
+			while (some == 0) {
+				from += 64 * 128;
+				if (from >= a.n) return a.n;
+				const int64_t at = from + lane * 128;
+				bool any = false;
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					if (at + 32 * i < a.n) any |= a.allow[(at >> 5) + i] != 0;
+				some = __ballot(any);
+			}
+			const int bit = __builtin_ctzll(some);
+			some &= some - 1;
+			return from + bit * 128;
+		};
 		Mx4Frag<KS> f, next;
-		load(wave * 32, next);
-		for (int64_t base = 0; base < a.n; base += 128) {
+		int64_t base = step();
+		load(base + wave * 32, next);
+		while (base < a.n) {
 			const int64_t row0 = base + wave * 32;
 			f = next;
-			load(row0 + 128, next);
+			base = step();
+			load(base + wave * 32, next);
 			if (row0 < a.n) {
 				mx4_shift_scales(f, half);
 				mx4_v16f acc[1];
@@ -945,13 +970,13 @@ __global__ __launch_bounds__(256) void mx4_rescue_kernel(Mx4Level a, int k, cons
 #pragma unroll
 				for (int i = 1; i < 16; i++) v = mx4_select(r32 == i, acc[0][i], v);
 				const int64_t id = row0 + 8 * (r32 >> 2) + 4 * half + (r32 & 3);
-				if (r32 < 16 && id < a.n && (!a.allow || ((a.allow[id >> 5] >> (id & 31)) & 1u))) {
+				if (r32 < 16 && id < a.n && (!FILTER || ((a.allow[id >> 5] >> (id & 31)) & 1u))) {
 					const mx4_key key = mx4_make_key(v, (unsigned)id);
 					if (key > least) keys[atomicAdd(&count, 1)] = key;
 				}
 			}
 			__syncthreads();
-			if (count > kMx4Gather - 128 || base + 128 >= a.n) {  // cut to the best
+			if (count > kMx4Gather - 128 || base >= a.n) {  // cut to the best
 				mx4_key key[kMx4Gather / 256];
 #pragma unroll
 				for (int j = 0; j < kMx4Gather / 256; j++) key[j] = j * 256 + tid < count ? keys[j * 256 + tid] : 0;
@@ -1150,8 +1175,10 @@ hipError_t mx4_scan_levels(const Mx4Plan &p, const uint8_t *q, int nq, const uin
 		else
 			pick(mx4_pick_kernel<256, kMx4GatherFewQueries, mx4_key, 4, 2>, mx4_key{}, nq);
 	}
-	if (p.levels)
-		hipLaunchKernelGGL((mx4_rescue_kernel<KS>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
+	if (p.levels && allow)
+		hipLaunchKernelGGL((mx4_rescue_kernel<KS, true>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
+	else if (p.levels)
+		hipLaunchKernelGGL((mx4_rescue_kernel<KS, false>), dim3(nq < 512 ? nq : 512), dim3(256), 0, s, a, k, over, last);
 	return hipGetLastError();
 }
 

@@ -148,3 +148,27 @@ def test_some_queries_overflow(engines, share):
     got, marked = scan_marked(mx, q, r, k, words)
     check(got, want_scan(mx, q, r, k, keep))
     assert marked[::3].all() and not marked[1::3].any() and not marked[2::3].any()
+
+
+@pytest.mark.parametrize("page", [32, 128, 3000, 20000])
+@pytest.mark.parametrize("nq,dim", [(12, 384), (300, 64), (300, 1000), (2200, 64)])
+def test_overflow_with_gaps(engines, nq, dim, page):
+    """Queries that are done over where the filter leaves out whole groups of rows, the store ending inside one of either kind."""
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(page)
+    mx, tiles, some = engines(dim), 1500, False
+    q = mx.quantize(1 + 0.5 * torch.randint(0, 2, (nq, dim), generator=g, device="cuda"))
+    order = torch.from_numpy(tile_order(tiles)).cuda()
+    good = torch.ones(tiles, dtype=torch.bool, device="cuda")
+    good[order[:215]] = False
+    for n, odd in ((64 * tiles, 0), (64 * tiles - 63, 1), (64 * tiles - 1, 0)):
+        at = torch.arange(n, device="cuda")
+        x = 1 + 0.5 * torch.randint(0, 2, (n, dim), generator=g, device="cuda")
+        x *= torch.where(good[at // 64], 1.0, -1.0)[:, None]
+        r = mx.quantize(x)
+        keep = (at // page) % 2 == odd
+        got, marked = scan_marked(mx, q, r, 10, words_of(keep))
+        check(got, want_scan(mx, q, r, 10, keep))
+        some |= bool(marked.any())
+    assert some
