@@ -259,7 +259,7 @@ size_t mvdb_mx4_scan_workspace(const mvdb_index *h, int nq, int n, int k);
 int mvdb_mx4_scan_many_dev(mvdb_index *h, const uint8_t *d_q, int nq, const uint8_t *d_rows, int n, int k, const uint32_t *d_allow,
                            int32_t *d_out_ids, float *d_out_val, int32_t *d_out_count, void *d_ws, size_t ws_bytes, void *stream);
 /* Host forms.  quantize: packed_out / values_out may each be NULL.  attach: quantise `rows` x dim f32 rows (row id = position, as
- * mvdb_attach_f32) into a store that the handle keeps in HBM; rows = 0 drops it.  product / scan: f32 queries against it. */
+ * mvdb_attach_f32) into a store that the handle keeps in HBM; rows = 0 drops it and frees its memory.  product / scan: f32 queries against it. */
 int mvdb_mx4_quantize(mvdb_index *h, const float *x, int64_t rows, uint8_t *packed_out, float *values_out);
 int mvdb_mx4_attach(mvdb_index *h, const float *base, int64_t rows);
 int64_t mvdb_mx4_rows(const mvdb_index *h);

@@ -58,6 +58,12 @@ struct DevBuf {
 		cap = want;
 		return p;
 	}
+	void release()
+	{
+		(void)hipFree(p);
+		p = nullptr;
+		cap = 0;
+	}
 };
 
 }  // namespace
@@ -1989,12 +1995,14 @@ int mvdb_mx4_attach(mvdb_index *h, const float *base, int64_t rows)
 {
 	const char *fn = "mvdb_mx4_attach";
 	if (rows < 0 || rows > INT32_MAX) return mx4_fail(h, fn, "row count out of range");
+	if (rows > 0 && !base) return mx4_fail(h, fn, "null pointer");
 	DeviceGuard dev(h);
 	if (!dev.ok) return 0;
 	const int dim = h->cfg.dim;
 	const size_t rb = mx4_row_bytes(dim);
 	h->mx4_n = 0;
-	if (!base || rows == 0) return 1;
+	if ((size_t)rows * rb < h->mx4_rows.cap / 2) h->mx4_rows.release();  // dropped, or much smaller than it was
+	if (rows == 0) return 1;
 	uint8_t *d_p = static_cast<uint8_t *>(h->mx4_rows.need((size_t)rows * rb));
 	if (!d_p) return mx4_fail(h, fn, "out of device memory (4-bit store)");
 	const int64_t chunk = std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)dim * 4));

@@ -1,0 +1,48 @@
+"""The 4-bit store that a handle keeps (mvdb_mx4_attach), and the memory that it takes."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _bridge(dim):
+    from minivectordb_amd import HipBridge
+    b = HipBridge(device=0)
+    b.init(dict(dim=dim, m=8, ef=50, capacity=8, seed=1))
+    return b
+
+
+def _free():
+    import torch
+    torch.cuda.synchronize()
+    return torch.cuda.mem_get_info()[0]
+
+
+def test_store_gives_its_memory_back(gpu):
+    """A store that is dropped, or takes the place of a much larger one, frees what it held: 96 MB here."""
+    b = _bridge(64)
+    x = np.random.default_rng(0).standard_normal((2_000_000, 64), dtype=np.float32)
+    b.mx4Attach(x)
+    assert b.mx4Rows() == len(x)
+    held = _free()
+    b.mx4Attach(x[:1000])
+    assert b.mx4Rows() == 1000 and _free() >= held + (90 << 20)
+    want = b.mx4ScanMany(x[:3], 5)
+    assert (want[0][:, 0] == [0, 1, 2]).all()
+    b.mx4Attach(x)
+    held = _free()
+    b.mx4Attach(None)
+    assert b.mx4Rows() == 0 and _free() >= held + (90 << 20)
+    b.mx4Attach(x[:1000])  # and it can be filled again
+    got = b.mx4ScanMany(x[:3], 5)
+    assert all(np.array_equal(a, c) for a, c in zip(got, want))
+    b.close()
+
+
+def test_refused_attach_keeps_the_store(gpu):
+    b = _bridge(64)
+    x = np.random.default_rng(1).standard_normal((100, 64), dtype=np.float32)
+    b.mx4Attach(x)
+    assert b._L.mvdb_mx4_attach(b.handle, None, 5) == 0 and b._L.mvdb_mx4_attach(b.handle, None, -1) == 0
+    assert b.mx4Rows() == 100 and (b.mx4ScanMany(x[:3], 5)[0][:, 0] == [0, 1, 2]).all()
+    b.close()
