@@ -2052,7 +2052,7 @@ int mvdb_mx4_product(mvdb_index *h, const float *q, int nq, float *out)
 	const size_t n = (size_t)h->mx4_n;
 	uint8_t *d_q = mx4_stage_queries(h, fn, q, nq);
 	if (!d_q) return 0;
-	const int64_t chunk = std::max<int64_t>(1, ((int64_t)1 << 30) / (int64_t)(n * 4));  // 1 GB of products at a time
+	const int64_t chunk = std::max<int64_t>(1, ((int64_t)256 << 20) / (int64_t)(n * 4));  // 256 MB of products at a time: the handle keeps the buffer
 	for (int64_t q0 = 0; q0 < nq; q0 += chunk) {
 		const int m = (int)std::min<int64_t>(chunk, nq - q0);
 		float *d_out = static_cast<float *>(h->st_mx4_ws.need((size_t)m * n * 4));

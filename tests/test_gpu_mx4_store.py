@@ -46,3 +46,16 @@ def test_refused_attach_keeps_the_store(gpu):
     assert b._L.mvdb_mx4_attach(b.handle, None, 5) == 0 and b._L.mvdb_mx4_attach(b.handle, None, -1) == 0
     assert b.mx4Rows() == 100 and (b.mx4ScanMany(x[:3], 5)[0][:, 0] == [0, 1, 2]).all()
     b.close()
+
+
+def test_host_product_keeps_little_memory(gpu):
+    """The handle keeps its staging of products between calls: 256 MB at most, and as much of f32 rows, however many products a call makes."""
+    b = _bridge(64)
+    x = np.random.default_rng(2).standard_normal((500_000, 64), dtype=np.float32)
+    b.mx4Attach(x)
+    b.mx4ProductMany(x[:1])  # (code and queries on the device)
+    held = _free()
+    out = b.mx4ProductMany(x[:300])  # 600 MB of products
+    assert held - _free() <= 260 << 20
+    assert np.array_equal(out[:140], b.mx4ProductMany(x[:140])) and np.array_equal(out[140:], b.mx4ProductMany(x[140:300]))
+    b.close()
