@@ -1054,7 +1054,9 @@ inline Mx4Plan mx4_plan(int nq, int n, int dim, int k)
 	p.first_rows = (int)((tiles + p.step0 - 1) / p.step0) * 64;
 	if (many) {
 		p.qtiles = (p.qgroups + 7) / 8;
-		p.splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles);  // 8 x qtiles workgroups at a time: one a compute unit
+		// 8 x qtiles workgroups at a time: one a compute unit, as long as there is a tile for each
+		const int64_t most_splits = 8 * (32 / p.qtiles < 1 ? 1 : 32 / p.qtiles), some = (tiles + 7) / 8 * 8;
+		p.splits = (int)(some < 8 ? 8 : some < most_splits ? some : most_splits);
 	} else {
 		const int wide = 32 * mx4_stream_frags(mx4_blocks(dim) / 2);
 		p.qgroups = (p.slab + wide - 1) / wide;
