@@ -246,6 +246,8 @@ class MiniVectorDB:
             self._mx4_dirty = False
         qn, _ = self.wasm.prepareQueries(qs)
         k = min(128, max(annK, topK))
+        words = (self.wasm.mx4Rows() + 31) // 32                  # a store opened with a smaller capacity: its rows past that are not allowed
+        allow = np.pad(allow, (0, max(0, words - allow.size)))
         cand, _, count = self.wasm.mx4ScanMany(qn, k, allow)
         return self.wasm.rerankMany(qn, cand, count, k, topK, allow)
 

@@ -59,3 +59,21 @@ def test_host_product_keeps_little_memory(gpu):
     assert held - _free() <= 260 << 20
     assert np.array_equal(out[:140], b.mx4ProductMany(x[:140])) and np.array_equal(out[140:], b.mx4ProductMany(x[140:300]))
     b.close()
+
+
+def test_database_opened_with_less_room(gpu, tmp_path):
+    """A store of 300 vectors opened again with room for 100: both kinds of candidates answer from the vectors that there is room for."""
+    from minivectordb_amd import MiniVectorDB
+    x = np.random.default_rng(0).standard_normal((300, 64)).astype(np.float32)
+    opts = dict(storageDir=str(tmp_path), dim=64, seed=1, preloadVectors=True)
+    db = MiniVectorDB.open(dict(opts, capacity=300))
+    db.insertMany([dict(id=f"d{i}", input=v) for i, v in enumerate(x)])
+    db.close()  # (without a snapshot of the graph, which would keep its room)
+    db = MiniVectorDB.open(dict(opts, capacity=100))
+    assert db.wasm.getMaxElements() == 100
+    xn = x.astype(np.float64) / np.linalg.norm(x.astype(np.float64), axis=1, keepdims=True)
+    for at in (3, 99, 250):
+        want = [f"d{i}" for i in np.argsort(np.square(xn[at] - xn[:100]).sum(1), kind="stable")[:5]]
+        for kind in ("graph", "mx4"):
+            assert [r["id"] for r in db.searchMany([x[at]], {"topK": 5, "candidates": kind})[0]] == want
+    db.close()
