@@ -240,10 +240,14 @@ int mvdb_scan_many_dev(mvdb_index *h, const int8_t *d_q, int nq, int k, int metr
  * up to a multiple of 16.  With m the largest magnitude of a block s = max(floor(log2 m) - 2, -127) + 127; a code is
  * the nearest to x / scale, ties to even, at most 6 in magnitude.  A block with a NaN or an infinity gets s = 255: every
  * product with it is NaN, and no scan returns it.
- * Products are summed in f32 by the matrix cores: exact while the scales of a row lie within a few powers of two of each other
- * (the products are small multiples of a power of two), otherwise off by an f32 rounding or two of the largest term.
- * `_dev` entry points take 16-byte aligned packed rows, allocate nothing, do not synchronise, may be captured into a graph and run
- * side by side on several streams (they keep nothing in the handle).  dim <= 4096, scans dim <= 1024 and k <= 128. */
+ * Products are summed in f32 by the matrix cores.  A product of two components is a multiple of 1/4 of its scales' product and at most
+ * 36 of it, so a sum is exact while 2 + log2(36 dim) + w <= 24, where the products of a query block's and a row block's scales lie within
+ * 2^w of each other (w <= 7.8 at dim 512, 4.8 at 4096); beyond that it is off by at most 65 (2^-24 P + 2^-149) for each 64 components, P
+ * = the sum of the products' magnitudes.  Where P passes the range of f32 the result may be infinite though the sum itself would fit; it is
+ * a NaN only where a block is one.
+ * `_dev` entry points take 16-byte aligned packed rows, allocate nothing, do not synchronise, may be captured into a graph, and their
+ * work may overlap on several streams: they keep nothing in the handle but, with mvdb_enable_timing on, the scans' event pairs (stage 3).
+ * As all `_dev` entry points they are issued from one host thread at a time.  dim <= 4096, scans dim <= 1024 and k <= 128. */
 int mvdb_mx4_row_bytes(const mvdb_index *h);
 /* rows x dim components of type dtype (0 f32, 1 bf16, 2 f16), ld components from one row to the next -> packed rows */
 int mvdb_mx4_quantize_dev(mvdb_index *h, const void *d_x, int dtype, int64_t rows, int64_t ld, uint8_t *d_packed, void *stream);

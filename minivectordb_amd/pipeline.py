@@ -213,7 +213,8 @@ class ResidentSearcher:
 class ResidentMx4:
     """The microscaled 4-bit operators over device tensors (mvdb_mx4_*_dev; the format is in include/mvdb_hip.h): rows -> packed
     rows, packed rows -> values, every dot product, the k largest dot products.  Everything runs on the caller's current
-    stream of `device`; nothing is kept between calls and nothing synchronises, so calls may be captured into a graph.
+    stream of `device`; nothing is kept between calls and nothing synchronises, so calls may be captured into a graph. Calls are made from one
+    thread at a time, as all device calls of a bridge; their work may overlap on several streams.
 
     A call on a few rows takes the GPU less time than the interpreter, so the methods check their arguments with as few
     steps as they can and pass plain numbers to the library."""
