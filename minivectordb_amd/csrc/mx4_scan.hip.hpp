@@ -5,7 +5,7 @@
 // and rows whose product is NaN are no candidates; a row is taken out by giving its blocks the scale 255, which makes every product NaN,
 // and a NaN is never >= a bound.
 //
-// Two ways, by the number of queries (1 M rows x 384, k 10: 8 queries 56 us in chunks, 9 queries 71 us in levels, 64 queries 79 us):
+// Two ways, by the number of queries (1 M rows x 384, k 10: 8 queries 56 us in chunks, 9 queries 72 us in levels, 64 queries 79 us):
 //
 // CHUNKS (up to 8 queries): a workgroup computes the products of its own run of rows, keeps them in LDS and picks the best k of each
 // query there; a second launch picks the best k of those.  Every row is read once, and two launches are all there is.
@@ -770,8 +770,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(Mx4Level a, int qgro
 // worked on the tiles of the next are asked for, one after the other.  One barrier a group: a wave that appends keeps the others waiting there, the
 // less the further the barriers are apart (4096 queries, 900 000 x 512, 168 candidates a query: barriers 1 tile apart 960 us, 2 tiles 880 us).
 // An image row is the packed row, plus one slot of 16 bytes where that makes the stride an odd number of slots: then the 16 lanes that an LDS read
-// serves at a time hit 16 different slots.  Two waves a SIMD.  4096 queries, 900 000 x 512: 725 us, 5.2 PFLOP/s (this card sustains 6.6 on random
-// operands); 1000 queries, x 384: 166 us, 4.2 PFLOP/s.
+// serves at a time hit 16 different slots.  Two waves a SIMD.  4096 queries, 900 000 x 512: 728-746 us, 5.1 PFLOP/s (this card sustains 6.6 on random
+// operands); 1000 queries, x 384: 167 us, 4.2 PFLOP/s.
 static __device__ __align__(16) int g_mx4_nan[4] = {-1, -1, -1, -1};  // scales 255: the blocks of a row that is left out
 
 __host__ __device__ constexpr int mx4_image_slots(int row_bytes) { return (row_bytes / 16) | 1; }
