@@ -248,15 +248,21 @@ hipError_t mx4_launch_product(const uint8_t *q, int nq, const uint8_t *rows, int
 			a.out = out + q0 * ldo;
 			const int frags = mx4_product_frags(ksteps);
 			a.groups = (a.nq + 32 * frags - 1) / (32 * frags);
-			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries (37 x 50 021 x 1000: two steps 9.4 us, one
-			// 11.1 us); but all of a small result's at once
+			// about kMx4ProductGroups workgroups, each with a run of steps that pays for its queries (37 x 50 021 x 1000: two steps 9.0 us, one
+			// 10.9 us; 1 to 256 queries, 5000 to 100 000 rows, dims 100 to 1000: two are up to 18 % faster where that makes more than 600
+			// workgroups, and nothing differs below); but all of a small result's at once
 			const int64_t run = rtiles * a.groups / kMx4ProductGroups, least = rtiles * a.groups >= 512 ? 2 : 1;
 			a.run = (int)(run < least ? least : run > 16 ? 16 : run);
 			const int64_t chunks = (rtiles + a.run - 1) / a.run;
 			const int64_t per_xcd = (chunks + 7) / 8, fit = kMx4BlockBytes / ((int64_t)a.run * 128 * row_bytes);
-			// With up to 16 groups the workgroups in flight spread over enough columns by themselves and share each row at once (1000 x 262 144 x
-			// 384: block 1 189 us, blocks of an L2 199); with 64 they do not (4096 x 65 536 x 512: 254 and 214).
-			a.block = (int)(a.groups <= 16 || fit < 1 ? 1 : fit < per_xcd ? fit : per_xcd);
+			// Blocks of an L2 or of one chunk, measured over 256 to 4096 queries, 40 000 to 524 288 rows, dims 100, 384, 1000 (times by blocks of one chunk
+			// / of an L2).  Many queries over result rows of moderate length write side by side only in blocks of an L2 (x 65 536 x 384: 1000 queries
+			// 71 / 56 us, 4096 243 / 216; 1000 to 4096 queries, 65 536 to 131 072 rows: 1.00 to 1.21).  Up to 512 queries, and over longer result rows, the
+			// workgroups in flight spread over enough columns by themselves and share each row at once (512 x 65 536 x 384 28 / 30 us, 512 x 262 144 x
+			// 384 102 / 115, 2048 x 262 144 x 384 398 / 451; 160 000 and 200 000 rows: 0.92 to 1.11).  Rows above dim 512, whose groups are half as large,
+			// gain nothing from them (x 1000: 0.89 to 1.01 with more than 1000 queries).
+			const bool blocks_of_l2 = ksteps <= 8 && a.groups > 8 && n < 150000 && fit >= 1;
+			a.block = (int)(blocks_of_l2 ? (fit < per_xcd ? fit : per_xcd) : 1);
 			const int64_t blocks = (per_xcd + a.block - 1) / a.block * a.block * 8 * a.groups;
 			mx4_for_steps(ksteps, [&](auto steps) {
 				constexpr int KS = decltype(steps)::value;
